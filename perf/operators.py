@@ -1,0 +1,344 @@
+"""What the learned layers between the features and the alignment cost: the cases that are measured.
+
+Three operators, in the directions a training step and a serving loop use them:
+
+  scan    the gated linear recurrence along every utterance of a ragged batch (srx_gated_scan_dev and its backward pass)
+  group   matrix products whose weights change from group to group of rows (srx_group_matmul_dev, its two gradients)
+  i8      8-bit matrix product with a scale for each row and each output (srx_quantize_rows_dev, srx_matmul_i8_dev)
+
+`own` False: the plain forms, in elementary torch operations.  `own` True: the library's entry points.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+SIZE = {"f32": 4, "f16": 2, "bf16": 2}
+
+
+# ------------------------------------------------------------------------------------------------- the cases
+def listed():
+    return [
+        # 32 live microphones, one new frame each: the state of every stream moves on by one step
+        dict(name="scan_step_32", op="scan", kind="sigmoid", dtype="f32", n=32, frames=32, dim=512, train=False, even=True),
+        # recursive smoothing of the 39 features of a 1,000-utterance batch (the batch of bench.py)
+        dict(name="scan_features_39", op="scan", kind="value", dtype="f32", n=1000, frames=499674, dim=39, train=False, even=False),
+        # one recurrent layer of 512 units over the same batch, forward and backward
+        dict(name="scan_train_512", op="scan", kind="sigmoid", dtype="bf16", n=1000, frames=499674, dim=512, train=True, even=False),
+        # one 20-minute recording in one piece, forward and backward
+        dict(name="scan_long_1024", op="scan", kind="value", dtype="f16", n=1, frames=120000, dim=1024, train=True, even=True),
+        # an affine transform of the 39 features for every utterance's own speaker
+        dict(name="group_speaker_39", op="group", dtype="f32", out="f32", n=1000, rows=499674, k=39, m=39, train=False),
+        # a serving step: 16 rows spread over 8 groups
+        dict(name="group_few_rows", op="group", dtype="bf16", out="bf16", n=8, rows=16, k=1024, m=1024, train=False),
+        # a layer of 16 groups over a batch of utterances
+        dict(name="group_forward", op="group", dtype="bf16", out="bf16", n=16, rows=32768, k=512, m=2048, train=False),
+        # 11 spliced frames of 39 features into 500 units, phone classes as groups: odd sizes, forward and backward
+        dict(name="group_train_odd", op="group", dtype="f16", out="f16", n=5, rows=10007, k=429, m=500, train=True),
+        # the largest training step of a layer
+        dict(name="group_train_1024", op="group", dtype="bf16", out="bf16", n=8, rows=65536, k=1024, m=1024, train=True),
+        # one frame of 4 streams against the 2,000 tied states
+        dict(name="i8_frames_4", op="i8", dtype="f32", out="f32", rows=4, k=512, m=2000, by_state=False),
+        # an utterance of odd sizes, scores laid out state by state as the alignment reads them
+        dict(name="i8_odd", op="i8", dtype="f16", out="f32", rows=4999, k=429, m=1999, by_state=True),
+        # scores of the 2,000 tied states for a batch of utterances
+        dict(name="i8_states_2000", op="i8", dtype="bf16", out="f32", rows=131072, k=1024, m=2000, by_state=False),
+    ]
+
+
+MOST = {"scan": 499674 * 512, "group": 65536 * 1024 * 1024, "i8": 131072 * 1024 * 2000}
+
+
+def _log(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    """One more case: sizes over their whole range by their logarithm, no dearer than the largest listed of its operator."""
+    op = rng.choice(["scan", "scan", "group", "group", "i8"])
+    dtype = rng.choice(["f32", "f16", "bf16"])
+    if op == "scan":
+        n, mean, dim = _log(rng, 1, 2000), _log(rng, 1, 20000), _log(rng, 1, 2048)
+        frames = max(1, min(n * mean, MOST[op] // dim, 499674))
+        return dict(op=op, kind=rng.choice(["sigmoid", "value"]), dtype=dtype, n=n, frames=frames, dim=dim, train=rng.random() < 0.5,
+                    even=False)
+    k, m, rows = _log(rng, 1, 2048), _log(rng, 1, 2048), _log(rng, 1, 131072)
+    rows = max(1, min(rows, MOST[op] // (k * m)))
+    if op == "group":
+        n = min(_log(rng, 1, 1000), max(1, (1 << 28) // (k * m)))
+        return dict(op=op, dtype=dtype, out=rng.choice([dtype, "f32"]), n=n, rows=rows, k=k, m=m, train=rng.random() < 0.5)
+    out = rng.choice(["f32", "f32", "f16", "bf16"])
+    return dict(op=op, dtype=dtype, out=out, rows=rows, k=k, m=m, by_state=rng.random() < 0.3)
+
+
+# ------------------------------------------------------------------------------------------------- inputs
+def _lengths(n, total, seed, even):
+    """n lengths that sum to total, 0.4 to 1.6 of their mean, and one in 16 (but not all) empty."""
+    if even:
+        return np.full(n, total // n, np.int64)
+    r = np.random.RandomState(seed)
+    w = r.uniform(0.4, 1.6, n) * (r.random_sample(n) >= 1 / 16)
+    if not w.any():
+        w[0] = 1.0
+    edge = np.floor(np.cumsum(w) / w.sum() * total + 0.5).astype(np.int64)
+    edge[np.flatnonzero(w)[-1]:] = total
+    return np.diff(edge, prepend=0)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed * 1000003 + 17)
+
+    def normal(*shape, scale=1.0, mean=0.0, dtype=torch.float32):
+        return (torch.randn(shape, generator=g, device="cuda") * scale + mean).to(dtype)
+
+    def empty(*shape, dtype=torch.float32):
+        return torch.zeros(shape, dtype=dtype, device="cuda")
+
+    s = dict(case)
+    t = TYPES[case["dtype"]]
+    if case["op"] == "i8":
+        rows, k, m, o = case["rows"], case["k"], case["m"], TYPES[case["out"]]
+        s["x"] = normal(rows, k, dtype=t)
+        # weights of a trained layer: normal, quantised once, a scale for each output
+        w = normal(m, k, scale=1 / math.sqrt(k))
+        s["ws"] = w.abs().amax(1).clamp_min(1e-30) / 127
+        s["wq"] = torch.round(w / s["ws"][:, None]).to(torch.int8)
+        s["bias"] = normal(m, scale=0.1)
+        # room that a serving loop keeps: codes in rows of whole 16 bytes, scales, scores
+        s["xq"], s["xs"] = empty(rows, -(-k // 16) * 16, dtype=torch.int8), empty(rows)
+        s["wq"] = torch.nn.functional.pad(s["wq"], (0, s["xq"].shape[1] - k))
+        s["y"] = empty(m, rows, dtype=o).t() if case["by_state"] else empty(rows, m, dtype=o)
+        return s
+    lens = _lengths(case["n"], case["frames" if case["op"] == "scan" else "rows"], seed, case.get("even", False))
+    total, n = int(lens.sum()), case["n"]
+    s["lens"] = lens
+    s["longest"] = int(lens.max())
+    s["off"] = torch.from_numpy(np.concatenate([[0], np.cumsum(lens)])).cuda()
+    if case["op"] == "scan":
+        dim = case["dim"]
+        s["live"] = torch.from_numpy(np.flatnonzero(lens)).cuda()
+        # gates of a trained layer: most of them keep the state for several frames
+        gate = normal(total, dim, scale=1.5, mean=2.0)
+        s["gate"] = (torch.sigmoid(gate) if case["kind"] == "value" else gate).to(t)
+        s["x"] = normal(total, dim, dtype=t)
+        s["h0"] = normal(n, dim, scale=0.3)
+        s["h"], s["h_last"] = empty(total, dim, dtype=t), empty(n, dim)
+        if case["train"]:
+            s["dh"], s["dh_last"] = normal(total, dim, dtype=t), normal(n, dim)
+            s["dgate"], s["dx"], s["dh0"] = empty(total, dim, dtype=t), empty(total, dim, dtype=t), empty(n, dim)
+        return s
+    k, m, o = case["k"], case["m"], TYPES[case["out"]]
+    s["x"] = normal(total, k, dtype=t)
+    s["w"] = normal(n, m, k, scale=1 / math.sqrt(k), dtype=t)
+    s["bias"] = normal(n, m, scale=0.1)
+    s["y"] = empty(total, m, dtype=o)
+    if case["train"]:
+        s["dy"] = normal(total, m, dtype=t)
+        s["dx"], s["dw"], s["dbias"] = empty(total, k, dtype=o), empty(n, m, k, dtype=o), empty(n, m)
+    return s
+
+
+def work(case):
+    z = SIZE[case["dtype"]]
+    if case["op"] == "scan":
+        e, state = case["frames"] * case["dim"], case["n"] * case["dim"] * 4
+        # gate and x read, h written; training reads the gradient of h and writes those of gate and x
+        return {"bytes": (6 if case["train"] else 3) * e * z + (4 if case["train"] else 2) * state, "flops": (10 if case["train"] else 3) * e}
+    rows, k, m, o = case["rows"], case["k"], case["m"], SIZE[case["out"]]
+    if case["op"] == "group":
+        n = case["n"]
+        b = rows * (k * z + m * o) + n * m * (k * z + 4)
+        if case["train"]:
+            b += rows * (m * z + k * o) + n * m * (k * o + 4)
+        return {"bytes": b, "flops": (6 if case["train"] else 2) * rows * k * m}
+    return {"bytes": rows * k * z + m * k + 8 * m + rows * m * o, "flops": 2 * rows * k * m}
+
+
+# ------------------------------------------------------------------------------------------------- one pass
+_kept = {}
+
+
+def _context():
+    """The context that a program keeps, on the device of the moment."""
+    if "ctx" not in _kept:
+        from speechrecognition_amd import host
+        _kept["host"], _kept["ctx"] = host, host.Context(torch.cuda.current_device())
+    return _kept["host"], _kept["ctx"]
+
+
+def _scratch(name, nbytes):
+    """Scratch memory that a program keeps from call to call, as large as the largest call so far needs."""
+    b = _kept.get(name)
+    if b is None or b.numel() < nbytes:
+        torch.cuda.synchronize()
+        b = _kept[name] = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device="cuda")
+    return b
+
+
+def run(s):
+    return {"scan": _scan, "group": _group, "i8": _i8}[s["op"]](s)
+
+
+def _doubling(a, h, longest):
+    """h_t = a_t h_(t-1) + h_t along the rows, where a is 0 in the first row of every stretch of at most `longest` rows: after the
+    step s every row holds its own last 2s terms."""
+    s = 1
+    while s < longest:
+        h = torch.cat([h[:s], torch.addcmul(h[s:], a[s:], h[:-s])])
+        a = torch.cat([a[:s], a[s:] * a[:-s]])
+        s *= 2
+    return h
+
+
+def _scan(s):
+    if own:
+        host, ctx = _context()
+        n, total, dim, longest = s["n"], s["x"].shape[0], s["dim"], s["longest"]
+        mode = host.SCAN_SIGMOID if s["kind"] == "sigmoid" else host.SCAN_VALUE
+        scratch = _scratch("scan", host.gated_scan_scratch_bytes(ctx, n, total, longest, dim))
+        states = _scratch("states", host.gated_scan_states_bytes(ctx, n, total, dim)) if s["train"] else None
+        host.gated_scan(ctx, mode, s["gate"], s["x"], s["off"], longest, s["h"], h0=s["h0"], h_last=s["h_last"], states=states,
+                        scratch=scratch)
+        if not s["train"]:
+            return {"h": s["h"], "h_last": s["h_last"]}
+        host.gated_scan_backward(ctx, mode, s["gate"], s["x"], s["off"], longest, states, s["dh"], s["dgate"], s["dx"],
+                                 dh_last=s["dh_last"], dh0=s["dh0"], scratch=scratch)
+        return {k: s[k] for k in ("h", "h_last", "dgate", "dx", "dh0")}
+    t = s["x"].dtype
+    live, x, gate = s["live"], s["x"].float(), s["gate"].float()
+    first, last = s["off"][live], s["off"][live + 1] - 1
+    a = torch.sigmoid(gate) if s["kind"] == "sigmoid" else gate
+    b = (1 - a) * x if s["kind"] == "sigmoid" else x + 0
+    b[first] += a[first] * s["h0"][live]
+    c = a.clone()
+    c[first] = 0
+    h = _doubling(c, b, s["longest"])
+    h_last = s["h0"].clone()
+    h_last[live] = h[last]
+    if not s["train"]:
+        return {"h": h.to(t), "h_last": h_last}
+    # the gradient runs the other way: lambda_t = dh_t + a_(t+1) lambda_(t+1)
+    c = torch.cat([a[1:], a[:1]])
+    c[last] = 0
+    d = s["dh"].to(torch.float32, copy=True)
+    d[last] += s["dh_last"][live]
+    lam = _doubling(c.flip(0), d.flip(0), s["longest"]).flip(0)
+    prev = torch.cat([h[:1], h[:-1]])
+    prev[first] = s["h0"][live]
+    if s["kind"] == "sigmoid":
+        dgate, dx = lam * (prev - x) * a * (1 - a), lam * (1 - a)
+    else:
+        dgate, dx = lam * prev, lam
+    dh0 = s["dh_last"].clone()
+    dh0[live] = a[first] * lam[first]
+    return {"h": h.to(t), "h_last": h_last, "dgate": dgate.to(t), "dx": dx.to(t), "dh0": dh0}
+
+
+def _padded(x, s):
+    """The rows group by group, [groups][longest][columns], zeros behind a group's last row, and where each row stands."""
+    row = torch.arange(x.shape[0], device=x.device)
+    group = torch.searchsorted(s["off"], row, right=True) - 1
+    at = row - s["off"][group]
+    p = torch.zeros((s["n"], s["longest"], x.shape[1]), dtype=torch.float32, device=x.device)
+    p[group, at] = x.float()
+    return p, group, at
+
+
+def _group(s):
+    if own:
+        host, ctx = _context()
+        host.group_matmul(ctx, s["x"], s["w"], s["off"], s["y"], bias=s["bias"])
+        if not s["train"]:
+            return {"y": s["y"]}
+        host.group_matmul_dx(ctx, s["dy"], s["w"], s["off"], s["dx"])
+        scratch = _scratch("group", host.group_matmul_dw_scratch_bytes(ctx, s["n"], s["x"].shape[0], s["k"], s["m"]))
+        host.group_matmul_dw(ctx, s["dy"], s["x"], s["off"], s["dw"], dbias=s["dbias"], scratch=scratch)
+        return {k: s[k] for k in ("y", "dx", "dw", "dbias")}
+    o = s["y"].dtype
+    x, group, at = _padded(s["x"], s)
+    w = s["w"].float()
+    y = torch.bmm(x, w.transpose(1, 2).contiguous()) + s["bias"][:, None]
+    y = y[group, at].to(o)
+    if not s["train"]:
+        return {"y": y}
+    dy, _, _ = _padded(s["dy"], s)
+    dx = torch.bmm(dy, w)[group, at].to(o)
+    dw = torch.bmm(dy.transpose(1, 2).contiguous(), x).to(o)
+    return {"y": y, "dx": dx, "dw": dw, "dbias": dy.sum(1)}
+
+
+def _i8(s):
+    if own:
+        host, ctx = _context()
+        host.quantize_rows(ctx, s["x"], s["xq"], s["xs"])
+        host.matmul_i8(ctx, s["xq"], s["xs"], s["wq"], s["ws"], s["k"], s["y"], bias=s["bias"])
+        return {"y": s["y"]}
+    x = s["x"].float()
+    scale = x.abs().amax(1, keepdim=True) / torch.full((1, 1), 127.0, device=x.device)
+    q = torch.where(scale > 0, torch.round(x / scale), 0.0)
+    y = torch.matmul(q, s["wq"][:, : s["k"]].float().t().contiguous())
+    return {"y": (y * scale * s["ws"] + s["bias"]).to(s["y"].dtype)}
+
+
+# ------------------------------------------------------------------------------------------------- in 64 bits
+def exact(case, seed):
+    """From the definitions, step by step and group by group, in 64 bits."""
+    s = prepare(case, seed)
+    if case["op"] == "i8":
+        # the code is the nearest whole number, ties to even, of the 32-bit quotient by the 32-bit scale; the rest is exact
+        x = s["x"].float().cpu()
+        scale = x.abs().amax(1) / torch.tensor([127.0])
+        q = torch.where(scale[:, None] > 0, torch.round(x / scale[:, None]), torch.zeros(()))
+        y = q.cuda().double() @ s["wq"][:, : case["k"]].double().t()
+        return {"y": y * scale.cuda().double()[:, None] * s["ws"].double() + s["bias"].double()}
+    off, n = s["off"].tolist(), case["n"]
+    if case["op"] == "group":
+        w, x = s["w"].double(), s["x"].double()
+        part = [slice(off[e], off[e + 1]) for e in range(n)]
+        out = {"y": torch.cat([x[p] @ w[e].t() + s["bias"][e].double() for e, p in enumerate(part)])}
+        if case["train"]:
+            dy = s["dy"].double()
+            out["dx"] = torch.cat([dy[p] @ w[e] for e, p in enumerate(part)])
+            out["dw"] = torch.stack([dy[p].t() @ x[p] for p in part])
+            out["dbias"] = torch.stack([dy[p].sum(0) for p in part])
+        return out
+    if s["longest"] > 130000:
+        return None
+    # time step by time step, the utterances side by side, longest first
+    order = np.argsort(-s["lens"], kind="stable")
+    lens, starts = s["lens"][order], s["off"].cpu().numpy()[:-1][order]
+    alive = [int(np.searchsorted(-lens, -t, side="left")) for t in range(s["longest"])]  # utterances longer than t
+    at = torch.from_numpy(starts.copy()).cuda()
+    a = s["gate"].double()
+    x = s["x"].double()
+    b = x
+    if case["kind"] == "sigmoid":
+        a = 1 / (1 + torch.exp(-a))
+        b = (1 - a) * x
+    idx = torch.from_numpy(order.copy()).cuda()
+    h, state = torch.empty_like(x), s["h0"].double()[idx]
+    prev = torch.empty_like(x) if case["train"] else None
+    for t in range(s["longest"]):
+        r = at[: alive[t]] + t
+        if prev is not None:
+            prev[r] = state[: alive[t]]
+        state[: alive[t]] = torch.addcmul(b[r], a[r], state[: alive[t]])
+        h[r] = state[: alive[t]]
+    h_last = torch.empty_like(state)
+    h_last[idx] = state
+    if not case["train"]:
+        return {"h": h, "h_last": h_last}
+    back, lam, dh = s["dh_last"].double()[idx], torch.empty_like(x), s["dh"].double()
+    for t in range(s["longest"] - 1, -1, -1):
+        r = at[: alive[t]] + t
+        v = dh[r] + back[: alive[t]]
+        lam[r] = v
+        back[: alive[t]] = a[r] * v
+    dh0 = torch.empty_like(back)
+    dh0[idx] = back
+    if case["kind"] == "sigmoid":
+        return {"h": h, "h_last": h_last, "dgate": lam * (prev - x) * a * (1 - a), "dx": lam * (1 - a), "dh0": dh0}
+    return {"h": h, "h_last": h_last, "dgate": lam * prev, "dx": lam, "dh0": dh0}

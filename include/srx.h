@@ -453,6 +453,45 @@ int srx_em_fused_dev(srx_ctx *ctx, srx_model *A, const float *feats_dev, int ld,
 int srx_em_fused_finish_dev(srx_ctx *ctx, srx_model *A, srx_model *B, const double *stats12_dev, const float *shift_dev,
                             float blend_keep, int32_t *underflow_dev);
 
+/* ---------------------------------------------------------------- learned layers -------- */
+/* Layers between the features and the emission scores that srx_viterbi_* reads, for models that are trained by their
+ * gradients.  NO COUNTERPART IN THE REFERENCE, whose emission model is the GMM.  Buffers are row-major device memory in one
+ * of three element types, row r at base + r * ld elements; sums, states, gates and scales are f32.  Every call is
+ * asynchronous on the context's stream, allocates nothing and keeps nothing between calls: scratch is the caller's, so calls
+ * may be captured into a graph (one scratch per graph that can run beside another).  Offset tables are DEVICE arrays and are
+ * held to [0, total] by the kernels.  Output buffers overlap no other buffer unless said so. */
+typedef enum { SRX_F32 = 0, SRX_F16 = 1, SRX_BF16 = 2 } srx_dtype;
+
+/* Gated linear recurrence along the frames of every utterance, channel by channel (beside the fixed smoothing of
+ * srx_features_batch_dev, over the same frame_off):
+ *   SRX_SCAN_VALUE    h_t = a_t h_(t-1) + x_t              a_t = gate_t
+ *   SRX_SCAN_SIGMOID  h_t = a_t h_(t-1) + (1 - a_t) x_t    a_t = 1 / (1 + exp(-gate_t))
+ * Utterance u owns frames [frame_off[u], frame_off[u+1]) and starts from h0[u] (h0_dev NULL: zeros); h_last[u] (h_last_dev
+ * NULL: not wanted) receives its last state, h0[u] for an utterance of no frames.  h_last may be h0: one call per new frame
+ * with frame_off = 0, 1, 2, ... moves every live stream on by one step.  Frames outside every utterance are left as they were.
+ * gate, x, h: [total_frames][ld >= D] of `dtype`; h0, h_last: [n_utt][D] f32.  The state is f32 throughout.
+ * max_frames: the longest utterance where the caller knows it (0: unknown); it only chooses how the work is cut.
+ * states_dev: srx_gated_scan_states_len floats that the backward pass reads (the state in front of every
+ * SRX_SCAN_STATE_EVERY-th frame), or NULL.  scratch_dev: srx_gated_scan_scratch_bytes (which may be 0), for either pass; it
+ * holds nothing between calls.  Where an utterance is cut into pieces its state passes a piece through the product of the
+ * piece's gates: for gates beyond +-1 that product has to stay inside the f32 range. */
+enum { SRX_SCAN_VALUE = 0, SRX_SCAN_SIGMOID = 1 };
+enum { SRX_SCAN_STATE_EVERY = 16 };
+int64_t srx_gated_scan_scratch_bytes(const srx_ctx *ctx, int n_utt, int64_t total_frames, int64_t max_frames, int D); /* -1: bad size */
+int64_t srx_gated_scan_states_len(const srx_ctx *ctx, int n_utt, int64_t total_frames, int D);                        /* -1: bad size */
+int srx_gated_scan_dev(srx_ctx *ctx, int mode, int dtype, const void *gate_dev, int64_t ld_gate, const void *x_dev, int64_t ld_x,
+                       const float *h0_dev, const int64_t *frame_off_dev, int n_utt, int64_t total_frames, int64_t max_frames, int D,
+                       void *h_dev, int64_t ld_h, float *h_last_dev, float *states_dev, void *scratch_dev, int64_t scratch_bytes);
+/* Its gradients.  dh: gradient of h; dh_last (or NULL: zeros): of h_last.  With lambda_t = dh_t + a_(t+1) lambda_(t+1) and
+ * dh_last behind the last frame: dx = lambda (VALUE) or lambda (1 - a); dgate = lambda h_(t-1) or
+ * lambda (h_(t-1) - x) a (1 - a), the gradient of the gate as it was passed; dh0 (or NULL) = a_first lambda_first, dh_last for
+ * an utterance of no frames.  dh0 may be dh_last.  gate, x, states and the sizes are those of the forward call. */
+int srx_gated_scan_backward_dev(srx_ctx *ctx, int mode, int dtype, const void *gate_dev, int64_t ld_gate, const void *x_dev, int64_t ld_x,
+                                const float *states_dev, const void *dh_dev, int64_t ld_dh, const float *dh_last_dev,
+                                const int64_t *frame_off_dev, int n_utt, int64_t total_frames, int64_t max_frames, int D,
+                                void *dgate_dev, int64_t ld_dgate, void *dx_dev, int64_t ld_dx, float *dh0_dev, void *scratch_dev,
+                                int64_t scratch_bytes);
+
 /* ---------------------------------------------------------------- multi-GPU exchange --- */
 /* One process per GPU, utterances sharded across the ranks; MFCC, scoring and alignment need no communication.  What
  * the ranks exchange are the sums that the reference's sequential loops over all utterances build:

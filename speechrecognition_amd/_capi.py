@@ -19,6 +19,12 @@ SRX_SCORE_MFMA = 0
 SRX_SCORE_EXACT = 1
 SRX_SCORE_MFMA_F16X3 = 2
 SRX_COMM_ID_BYTES = 128
+SRX_F32 = 0
+SRX_F16 = 1
+SRX_BF16 = 2
+SRX_SCAN_VALUE = 0
+SRX_SCAN_SIGMOID = 1
+SRX_SCAN_STATE_EVERY = 16
 
 
 class SrxError(RuntimeError):
@@ -125,6 +131,11 @@ SIGNATURES = {
     "srx_em_fused_len": (i64, [vp]),
     "srx_em_fused_dev": (C.c_int, [vp, vp, vp, C.c_int, vp, i64, vp, vp, vp]),
     "srx_em_fused_finish_dev": (C.c_int, [vp, vp, vp, vp, vp, C.c_float, vp]),
+    "srx_gated_scan_scratch_bytes": (i64, [vp, C.c_int, i64, i64, C.c_int]),
+    "srx_gated_scan_states_len": (i64, [vp, C.c_int, i64, C.c_int]),
+    "srx_gated_scan_dev": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, vp, i64, vp, vp, C.c_int, i64, i64, C.c_int, vp, i64, vp, vp, vp, i64]),
+    "srx_gated_scan_backward_dev": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, vp, i64, vp, vp, i64, vp, vp, C.c_int, i64, i64, C.c_int,
+                                              vp, i64, vp, i64, vp, vp, i64]),
     "srx_comm_unique_id": (C.c_int, [vp]),
     "srx_comm_create": (C.c_int, [vp, C.c_int, C.c_int, vp, C.POINTER(vp)]),
     "srx_comm_create_host": (C.c_int, [vp, C.c_int, C.c_int, C.c_char_p, C.POINTER(vp)]),

@@ -584,6 +584,117 @@ def gather_gid(ctx, hmm, path_d, status_d):
     return gid
 
 
+# ----------------------------------------------------------------------------- learned layers
+# Device buffers of these calls are DevArrays (bf16 held as uint16) or torch tensors on the context's device.  The library's
+# calls are asynchronous on the context's stream: a tensor that another stream writes or reads is ordered by the caller.
+SCAN_VALUE, SCAN_SIGMOID = _capi.SRX_SCAN_VALUE, _capi.SRX_SCAN_SIGMOID
+_DTYPES = {"float32": _capi.SRX_F32, "float16": _capi.SRX_F16, "uint16": _capi.SRX_BF16, "bfloat16": _capi.SRX_BF16, "int8": "i8",
+           "int64": "i64", "uint8": "u8"}
+
+
+def _typed(a):
+    """Element type of a DevArray or a torch tensor: SRX_F32 / SRX_F16 / SRX_BF16, or "i8" / "i64" / "u8"."""
+    t = _DTYPES.get(a.dtype)
+    if t is None:
+        t = _DTYPES.get(str(a.dtype).replace("torch.", ""))
+        if t is None:
+            raise ValueError(f"element type {a.dtype} is not supported")
+        _DTYPES[a.dtype] = t
+    return t
+
+
+def _buf(a, ctx):
+    """Device address of a DevArray or a torch tensor (None: null)."""
+    if a is None:
+        return None
+    if hasattr(a, "data_ptr"):
+        if a.device.type != "cuda" or a.device.index != ctx.device:
+            raise ValueError(f"a tensor on {a.device}: the context works on device {ctx.device}")
+        return a.data_ptr()
+    return a.ptr
+
+
+def _strides(a):
+    if hasattr(a, "data_ptr"):
+        return a.stride()
+    s, r = [], 1
+    for n in reversed(a.shape):
+        s.append(r)
+        r *= n
+    return tuple(reversed(s))
+
+
+def _rows(a, rows, cols, dtype, what, ctx):
+    """(address, row stride) of a [rows][cols] matrix with adjacent columns."""
+    st = _strides(a)
+    if tuple(a.shape) != (rows, cols) or _typed(a) != dtype or (cols > 1 and st[1] != 1) or (rows > 1 and st[0] < cols):
+        raise ValueError(f"{what}: {tuple(a.shape)} {a.dtype} with strides {tuple(st)}, wanted [{rows}][{cols}] of one type with adjacent columns")
+    return _buf(a, ctx), max(st[0], cols)
+
+
+def _dense(a, shape, dtype, what, ctx):
+    """Address of a contiguous array of that shape and type, or of one with as many elements in a single dimension."""
+    if a is None:
+        return None
+    n = 1
+    for v in shape:
+        n *= v
+    if (tuple(a.shape) != tuple(shape) and tuple(a.shape) != (n,)) or _typed(a) != dtype or (hasattr(a, "data_ptr") and not a.is_contiguous()):
+        raise ValueError(f"{what}: {tuple(a.shape)} {a.dtype}, wanted contiguous {tuple(shape)}")
+    return _buf(a, ctx)
+
+
+def _room(a, ctx):
+    """(address, bytes) of a caller's scratch or state buffer."""
+    if a is None:
+        return None, 0
+    return _buf(a, ctx), a.nbytes if isinstance(a, DevArray) else a.numel() * a.element_size()
+
+
+def gated_scan_scratch_bytes(ctx, n_utt, total_frames, max_frames, D):
+    return ctx.lib.srx_gated_scan_scratch_bytes(ctx.h, n_utt, total_frames, max_frames, D)
+
+
+def gated_scan_states_bytes(ctx, n_utt, total_frames, D):
+    return 4 * ctx.lib.srx_gated_scan_states_len(ctx.h, n_utt, total_frames, D)
+
+
+def gated_scan(ctx, mode, gate, x, frame_off, max_frames, h, h0=None, h_last=None, states=None, scratch=None):
+    """h_t = a_t h_(t-1) + x_t (SCAN_VALUE, a = gate) or a_t h_(t-1) + (1 - a_t) x_t (SCAN_SIGMOID, a = sigmoid(gate)) along every
+    utterance: gate, x -> h [T][D]; h0 -> h_last [n_utt][D] f32.  states (gated_scan_states_bytes): for gated_scan_backward."""
+    T, D = x.shape
+    n, t = frame_off.shape[0] - 1, _typed(x)
+    g, ldg = _rows(gate, T, D, t, "gate", ctx)
+    xp, ldx = _rows(x, T, D, t, "x", ctx)
+    hp, ldh = _rows(h, T, D, t, "h", ctx)
+    sp, sn = _room(states, ctx)
+    if states is not None and sn < gated_scan_states_bytes(ctx, n, T, D):
+        raise ValueError(f"states: {sn} bytes, {gated_scan_states_bytes(ctx, n, T, D)} needed")
+    wp, wn = _room(scratch, ctx)
+    check(ctx.lib.srx_gated_scan_dev(ctx.h, mode, t, g, ldg, xp, ldx, _dense(h0, (n, D), 0, "h0", ctx), _dense(frame_off, (n + 1,), "i64", "frame_off", ctx),
+                                     n, T, max_frames, D, hp, ldh, _dense(h_last, (n, D), 0, "h_last", ctx), sp, wp, wn), ctx.h)
+    return h
+
+
+def gated_scan_backward(ctx, mode, gate, x, frame_off, max_frames, states, dh, dgate, dx, dh_last=None, dh0=None, scratch=None):
+    """Gradients of gated_scan: dh [T][D] (and dh_last [n_utt][D]) -> dgate, dx [T][D] (and dh0 [n_utt][D])."""
+    T, D = x.shape
+    n, t = frame_off.shape[0] - 1, _typed(x)
+    g, ldg = _rows(gate, T, D, t, "gate", ctx)
+    xp, ldx = _rows(x, T, D, t, "x", ctx)
+    dp, ldd = _rows(dh, T, D, t, "dh", ctx)
+    gp, ldgp = _rows(dgate, T, D, t, "dgate", ctx)
+    op, ldo = _rows(dx, T, D, t, "dx", ctx)
+    sp, sn = _room(states, ctx)
+    if sn < gated_scan_states_bytes(ctx, n, T, D):
+        raise ValueError(f"states: {sn} bytes, {gated_scan_states_bytes(ctx, n, T, D)} needed")
+    wp, wn = _room(scratch, ctx)
+    check(ctx.lib.srx_gated_scan_backward_dev(ctx.h, mode, t, g, ldg, xp, ldx, sp, dp, ldd, _dense(dh_last, (n, D), 0, "dh_last", ctx),
+                                              _dense(frame_off, (n + 1,), "i64", "frame_off", ctx), n, T, max_frames, D, gp, ldgp, op, ldo,
+                                              _dense(dh0, (n, D), 0, "dh0", ctx), wp, wn), ctx.h)
+    return dgate, dx
+
+
 # ----------------------------------------------------------------------------- multi-GPU exchange
 class Comm:
     """srx_comm: the all-reduces of sufficient statistics behind the C ABI (RCCL; world 1 = no-ops)."""

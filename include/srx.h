@@ -492,6 +492,39 @@ int srx_gated_scan_backward_dev(srx_ctx *ctx, int mode, int dtype, const void *g
                                 void *dgate_dev, int64_t ld_dgate, void *dx_dev, int64_t ld_dx, float *dh0_dev, void *scratch_dev,
                                 int64_t scratch_bytes);
 
+/* Matrix products whose weights change from group to group of rows (speakers, utterances, phone classes; beside
+ * alignment-mode scoring, where every utterance meets its own states).  Group e owns rows [row_off[e], row_off[e+1]) (DEVICE
+ * array of n_groups + 1 entries, frame_off's form); a group may have none.  W: [n_groups][N][K] contiguous, of the rows' type.
+ *   srx_group_matmul_dev      y_r = W_e x_r + b_e            x [total_rows][ld >= K] -> y [total_rows][ld >= N]; bias [n_groups][N] f32 or NULL
+ *   srx_group_matmul_dx_dev   dx_r = W_e^T dy_r              dy [total_rows][ld >= N] -> dx [total_rows][ld >= K]
+ *   srx_group_matmul_dw_dev   dW_e = sum dy_r x_r^T          -> dw [n_groups][N][K], zeros for a group of no rows;
+ *                             db_e = sum dy_r                -> dbias [n_groups][N] f32, or NULL
+ * in_dtype: f32, f16 or bf16 (products on the matrix cores of that type, sums in f32); out_dtype: the same or f32.  Rows of no
+ * group are left as they were.  Results do not depend on the order in which the workgroups run. */
+int srx_group_matmul_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *x_dev, int64_t ld_x, const void *w_dev, const float *bias_dev,
+                         const int64_t *row_off_dev, int n_groups, int64_t total_rows, int K, int N, void *y_dev, int64_t ld_y);
+int srx_group_matmul_dx_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *w_dev, const int64_t *row_off_dev,
+                            int n_groups, int64_t total_rows, int K, int N, void *dx_dev, int64_t ld_dx);
+int64_t srx_group_matmul_dw_scratch_bytes(const srx_ctx *ctx, int n_groups, int64_t total_rows, int K, int N); /* may be 0; -1: bad size */
+int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *x_dev, int64_t ld_x,
+                            const int64_t *row_off_dev, int n_groups, int64_t total_rows, int K, int N, void *dw_dev, float *dbias_dev,
+                            void *scratch_dev, int64_t scratch_bytes);
+
+/* 8-bit matrix product with a scale for each row and each output (beside srx_gmm_score_dev: emission scores of an output layer
+ * over the tied states, in the strides that srx_viterbi_* reads).
+ * srx_quantize_rows_dev: scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded to the nearest whole
+ *   number, ties to even; a row of zeros has scale 0 and codes 0; a row that holds a NaN or an infinity has that as its scale
+ *   and codes 0, so that its outputs are NaN.  x: [rows][ld >= K] of `dtype`; codes: [rows][ld_q], ld_q a multiple of 16 bytes,
+ *   q_dev 16-byte aligned, zeros written behind column K up to whole 16 bytes.  Weights (rows = outputs) are quantised by the
+ *   same call, once.
+ * srx_matmul_i8_dev: y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n (the sum exact in 32 bits; bias f32 or NULL) at
+ *   y[r * stride_r + n * stride_n], one of the two strides 1 (row by row: stride_n = 1; state by state: stride_r = 1), of
+ *   out_dtype.  Codes may come from elsewhere: at least one operand has to hold zeros behind column K up to whole 16 bytes. */
+enum { SRX_I8_MAX_K = 131072 };
+int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev, int64_t ld_x, int64_t rows, int K, int8_t *q_dev, int64_t ld_q, float *scale_dev);
+int srx_matmul_i8_dev(srx_ctx *ctx, int out_dtype, const int8_t *xq_dev, int64_t ld_xq, const float *xs_dev, const int8_t *wq_dev, int64_t ld_wq,
+                      const float *ws_dev, const float *bias_dev, int64_t rows, int N, int K, void *y_dev, int64_t stride_r, int64_t stride_n);
+
 /* ---------------------------------------------------------------- multi-GPU exchange --- */
 /* One process per GPU, utterances sharded across the ranks; MFCC, scoring and alignment need no communication.  What
  * the ranks exchange are the sums that the reference's sequential loops over all utterances build:

@@ -25,6 +25,7 @@ SRX_BF16 = 2
 SRX_SCAN_VALUE = 0
 SRX_SCAN_SIGMOID = 1
 SRX_SCAN_STATE_EVERY = 16
+SRX_I8_MAX_K = 131072
 
 
 class SrxError(RuntimeError):
@@ -136,6 +137,12 @@ SIGNATURES = {
     "srx_gated_scan_dev": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, vp, i64, vp, vp, C.c_int, i64, i64, C.c_int, vp, i64, vp, vp, vp, i64]),
     "srx_gated_scan_backward_dev": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, vp, i64, vp, vp, i64, vp, vp, C.c_int, i64, i64, C.c_int,
                                               vp, i64, vp, i64, vp, vp, i64]),
+    "srx_group_matmul_dev": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, vp, vp, vp, C.c_int, i64, C.c_int, C.c_int, vp, i64]),
+    "srx_group_matmul_dx_dev": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, vp, vp, C.c_int, i64, C.c_int, C.c_int, vp, i64]),
+    "srx_group_matmul_dw_scratch_bytes": (i64, [vp, C.c_int, i64, C.c_int, C.c_int]),
+    "srx_group_matmul_dw_dev": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, vp, i64, vp, C.c_int, i64, C.c_int, C.c_int, vp, vp, vp, i64]),
+    "srx_quantize_rows_dev": (C.c_int, [vp, C.c_int, vp, i64, i64, C.c_int, vp, i64, vp]),
+    "srx_matmul_i8_dev": (C.c_int, [vp, C.c_int, vp, i64, vp, vp, i64, vp, vp, i64, C.c_int, C.c_int, vp, i64, i64]),
     "srx_comm_unique_id": (C.c_int, [vp]),
     "srx_comm_create": (C.c_int, [vp, C.c_int, C.c_int, vp, C.POINTER(vp)]),
     "srx_comm_create_host": (C.c_int, [vp, C.c_int, C.c_int, C.c_char_p, C.POINTER(vp)]),

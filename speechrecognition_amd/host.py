@@ -695,6 +695,84 @@ def gated_scan_backward(ctx, mode, gate, x, frame_off, max_frames, states, dh, d
     return dgate, dx
 
 
+def _weights(w, n, dtype, what, ctx):
+    if len(w.shape) != 3 or w.shape[0] != n:
+        raise ValueError(f"{what}: {tuple(w.shape)}, wanted [{n}][outputs][inputs]")
+    return _dense(w, tuple(w.shape), dtype, what, ctx)
+
+
+def group_matmul(ctx, x, w, row_off, y, bias=None):
+    """y_r = W_e x_r + b_e for the rows r of group e: x [T][K], w [E][N][K], bias [E][N] f32 -> y [T][N] (x's type or f32)."""
+    (T, K), E, t = x.shape, row_off.shape[0] - 1, _typed(x)
+    N = w.shape[1]
+    xp, ldx = _rows(x, T, K, t, "x", ctx)
+    yp, ldy = _rows(y, T, N, _typed(y), "y", ctx)
+    if w.shape[2] != K:
+        raise ValueError(f"w: {tuple(w.shape)}, wanted [{E}][{N}][{K}]")
+    check(ctx.lib.srx_group_matmul_dev(ctx.h, t, _typed(y), xp, ldx, _weights(w, E, t, "w", ctx), _dense(bias, (E, N), 0, "bias", ctx),
+                                       _dense(row_off, (E + 1,), "i64", "row_off", ctx), E, T, K, N, yp, ldy), ctx.h)
+    return y
+
+
+def group_matmul_dx(ctx, dy, w, row_off, dx):
+    """dx_r = W_e^T dy_r: dy [T][N], w [E][N][K] -> dx [T][K] (dy's type or f32)."""
+    (T, N), E, t = dy.shape, row_off.shape[0] - 1, _typed(dy)
+    K = w.shape[2]
+    dp, ldd = _rows(dy, T, N, t, "dy", ctx)
+    op, ldo = _rows(dx, T, K, _typed(dx), "dx", ctx)
+    if w.shape[1] != N:
+        raise ValueError(f"w: {tuple(w.shape)}, wanted [{E}][{N}][{K}]")
+    check(ctx.lib.srx_group_matmul_dx_dev(ctx.h, t, _typed(dx), dp, ldd, _weights(w, E, t, "w", ctx), _dense(row_off, (E + 1,), "i64", "row_off", ctx),
+                                          E, T, K, N, op, ldo), ctx.h)
+    return dx
+
+
+def group_matmul_dw_scratch_bytes(ctx, n_groups, total_rows, K, N):
+    return ctx.lib.srx_group_matmul_dw_scratch_bytes(ctx.h, n_groups, total_rows, K, N)
+
+
+def group_matmul_dw(ctx, dy, x, row_off, dw, dbias=None, scratch=None):
+    """dW_e = sum of dy_r x_r^T, db_e = sum of dy_r over the rows of group e: dy [T][N], x [T][K] -> dw [E][N][K], dbias [E][N] f32."""
+    (T, N), E, t = dy.shape, row_off.shape[0] - 1, _typed(dy)
+    K = x.shape[1]
+    dp, ldd = _rows(dy, T, N, t, "dy", ctx)
+    xp, ldx = _rows(x, T, K, t, "x", ctx)
+    wp, wn = _room(scratch, ctx)
+    check(ctx.lib.srx_group_matmul_dw_dev(ctx.h, t, _typed(dw), dp, ldd, xp, ldx, _dense(row_off, (E + 1,), "i64", "row_off", ctx), E, T, K, N,
+                                          _dense(dw, (E, N, K), _typed(dw), "dw", ctx), _dense(dbias, (E, N), 0, "dbias", ctx), wp, wn), ctx.h)
+    return dw
+
+
+def quantize_rows(ctx, x, q, scale):
+    """scale_r = max |x_r| / 127, q_r = round(x_r / scale_r): x [T][K] -> codes q [T][>= K, whole 16 bytes] int8, scale [T] f32."""
+    T, K = x.shape
+    xp, ldx = _rows(x, T, K, _typed(x), "x", ctx)
+    qp, ldq = _rows(q, T, q.shape[1], "i8", "q", ctx)
+    if q.shape[1] < (K + 15) // 16 * 16:
+        raise ValueError(f"q: {tuple(q.shape)}, wanted [{T}][{(K + 15) // 16 * 16}]")
+    check(ctx.lib.srx_quantize_rows_dev(ctx.h, _typed(x), xp, ldx, T, K, qp, ldq, _dense(scale, (T,), 0, "scale", ctx)), ctx.h)
+    return q, scale
+
+
+def matmul_i8(ctx, xq, xs, wq, ws, K, y, bias=None):
+    """y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n: codes xq [T][>= K], wq [N][>= K] int8, scales f32 -> y [T][N] (also a
+    transposed view: scores state by state)."""
+    T, N = xq.shape[0], wq.shape[0]
+    k16 = (K + 15) // 16 * 16
+    xp, ldx = _rows(xq, T, xq.shape[1], "i8", "xq", ctx)
+    wp, ldw = _rows(wq, N, wq.shape[1], "i8", "wq", ctx)
+    if xq.shape[1] < k16 or wq.shape[1] < k16 or tuple(y.shape) != (T, N):
+        raise ValueError(f"codes {tuple(xq.shape)}, {tuple(wq.shape)}, scores {tuple(y.shape)} for K = {K}")
+    sr, sn = _strides(y)
+    if sn == 1 or N == 1:
+        sr, sn = max(sr, N) if T == 1 else sr, 1
+    elif T == 1:
+        sr, sn = 1, max(sn, T)
+    check(ctx.lib.srx_matmul_i8_dev(ctx.h, _typed(y), xp, ldx, _dense(xs, (T,), 0, "xs", ctx), wp, ldw, _dense(ws, (N,), 0, "ws", ctx),
+                                    _dense(bias, (N,), 0, "bias", ctx), T, N, K, _buf(y, ctx), sr, sn), ctx.h)
+    return y
+
+
 # ----------------------------------------------------------------------------- multi-GPU exchange
 class Comm:
     """srx_comm: the all-reduces of sufficient statistics behind the C ABI (RCCL; world 1 = no-ops)."""

@@ -68,3 +68,48 @@ def scan_back(f, g, x, off, dh, dlast, sigmoid):
     dg = lam * w * diff
     return dict(dx=dx, edx=el * na + np.abs(dx) * (ra + 3 * U), dg=dg,
                 edg=el * w * np.abs(diff) + np.abs(lam) * w * ediff + np.abs(dg) * (2 * ra + 6 * U), d0=d0, e0=e0)
+
+
+def product(p, q, dtype):
+    """p @ q in 64 bits (p, q hold exact values of the operands' type) and the bound of an f32 accumulation in any order:
+    every product is exact (16-bit types) or half a step off (f32), every one of the k - 1 additions half a step of a partial
+    sum that is at most sum |p| |q|."""
+    mag = np.abs(p) @ np.abs(q)
+    k = p.shape[1]
+    return p @ q, U * (k + 1) * mag
+
+
+def group(x, w, off, bias, dtype):
+    y, e = np.zeros((x.shape[0], w.shape[1])), np.zeros((x.shape[0], w.shape[1]))
+    for g in range(len(off) - 1):
+        r = slice(off[g], off[g + 1])
+        v, b = product(x[r], w[g].T, dtype)
+        y[r], e[r] = (v, b) if bias is None else (v + bias[g], b + U * np.abs(v + bias[g]))
+    return y, e
+
+
+def group_dw(dy, x, off, dtype):
+    n = len(off) - 1
+    dw, e = np.zeros((n, dy.shape[1], x.shape[1])), np.zeros((n, dy.shape[1], x.shape[1]))
+    db, eb = np.zeros((n, dy.shape[1])), np.zeros((n, dy.shape[1]))
+    for g in range(n):
+        r = slice(off[g], off[g + 1])
+        dw[g], e[g] = product(dy[r].T, x[r], dtype)
+        db[g], eb[g] = dy[r].sum(0), U * (off[g + 1] - off[g]) * np.abs(dy[r]).sum(0)
+    return dw, e, db, eb
+
+
+def quantize(x):
+    """Scale and codes by definition: f32 maximum / 127, f32 quotient, nearest whole number, ties to even."""
+    x = np.asarray(x, np.float32)
+    s = np.abs(x).max(1) / np.float32(127)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        q = np.rint((x / s[:, None]).astype(np.float32))
+    return s, np.where(np.isfinite(s[:, None]) & (s[:, None] > 0), q, 0).astype(np.int8)
+
+
+def i8(xq, xs, wq, ws, bias):
+    """The sum is exact; its rounding to f32, two scales, the bias: four half steps."""
+    v = (xq.astype(np.int64) @ wq.astype(np.int64).T) * xs[:, None].astype(np.float64) * ws.astype(np.float64)
+    y = v if bias is None else v + bias.astype(np.float64)
+    return y, 3.01 * U * np.abs(v) + U * np.abs(y)

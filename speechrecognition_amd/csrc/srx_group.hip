@@ -8,6 +8,8 @@
 // the output unit (dW).  Groups are ragged and known on the device only: row tile number t of the launch belongs to the group e
 // with row_off[e] / TJ + e <= t < row_off[e+1] / TJ + e + 1, a closed form that needs no table (the range holds at least the
 // ceil(rows / TJ) tiles that group e needs; the spare ones leave at once).
+#include <type_traits>
+
 #include "srx_tile.h"
 
 struct GroupArgs {
@@ -54,9 +56,9 @@ template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, bool DMA>
 __global__ __launch_bounds__(WI *WJ * 64) void k_group(GroupArgs p) {
     typedef Tile<El, WI, WJ, FI, FJ, DX, false, DMA> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
-    const int64_t item = xcd_item(blockIdx.x, p.tiles_i * p.tiles_j);
-    const int64_t tj = item / p.tiles_i;
-    const int i0 = (int)(item - tj * p.tiles_i) * T::TI;
+    int64_t ti, tj;
+    tile_of(blockIdx.x, p.tiles_i, p.tiles_j, ti, tj);
+    const int i0 = (int)ti * T::TI;
     int e, rows;
     int64_t r0;
     if (!group_rows<T::TJ>(p, tj, e, r0, rows)) return;
@@ -74,14 +76,44 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_group(GroupArgs p) {
     float none[FJ];
     T::template product<false>(smem, P, Q, R, acc, none, false);
     O *y = reinterpret_cast<O *>(p.y);
-    const bool aligned = (p.ld_y % 4 == 0) && (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(O)) == 0);
     const float *bias = !DX && p.bias ? p.bias + (int64_t)e * p.N : nullptr;
-    T::each(acc, [&](int i, int j, const auto &v) {
-        if (j >= rows || i0 + i >= I) return;
+    struct Held { float b[RUN<O>]; };
+    T::template write_out<RUN<O>>(
+        smem, acc,
+        [&](int i) {
+            Held h;
+#pragma unroll
+            for (int q = 0; q < RUN<O>; q++) h.b[q] = bias && i0 + i + q < I ? bias[i0 + i + q] : 0.0f;
+            return h;
+        },
+        [&](int i, int j, const float (&v)[RUN<O>], const Held &h) {
+            if (j >= rows || i0 + i >= I) return;
+            float f[RUN<O>];
+#pragma unroll
+            for (int q = 0; q < RUN<O>; q++) f[q] = v[q] + h.b[q];
+            store_run<O>(y + (r0 + j) * p.ld_y + i0 + i, f, I - i0 - i);
+        });
+}
+
+// forward, few rows per group: tiles of 32 x 32
+template <class El, class O>
+__global__ __launch_bounds__(THIN_WAVES * 64) void k_group_thin(GroupArgs p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[THIN_LDS];
+    const int i0 = (int)(blockIdx.x % p.tiles_i) * 32;
+    int e, rows;
+    int64_t r0;
+    if (!group_rows<32>(p, blockIdx.x / p.tiles_i, e, r0, rows)) return;
+    const El *w = reinterpret_cast<const El *>(p.w) + ((int64_t)e * p.N + i0) * p.K;
+    const TileOperand P{w, p.K, p.N - i0 < 32 ? p.N - i0 : 32};
+    const TileOperand Q{reinterpret_cast<const El *>(p.x) + r0 * p.ld_x, p.ld_x, rows};
+    O *y = reinterpret_cast<O *>(p.y);
+    const float *bias = p.bias ? p.bias + (int64_t)e * p.N : nullptr;
+    thin_product<El>(smem, P, Q, p.K, [&](int i, int j, const float (&v)[4]) {
+        if (j >= rows || i0 + i >= p.N) return;
         float f[4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) f[q] = v[q] + (bias && i0 + i + q < I ? bias[i0 + i + q] : 0.0f);
-        store4<O>(y + (r0 + j) * p.ld_y + i0 + i, f, I - i0 - i, aligned);
+        for (int q = 0; q < 4; q++) f[q] = v[q] + (bias && i0 + i + q < p.N ? bias[i0 + i + q] : 0.0f);
+        store_four<O>(y + (r0 + j) * p.ld_y + i0 + i, f, p.N - i0 - i);
     });
 }
 
@@ -91,9 +123,9 @@ template <class El, class O, int WI, int WJ, int FI, int FJ, bool DMA>
 __global__ __launch_bounds__(WI *WJ * 64) void k_group_dw(GroupArgs p) {
     typedef Tile<El, WI, WJ, FI, FJ, true, true, DMA> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
-    const int64_t item = xcd_item(blockIdx.x, p.tiles_i * p.tiles_j);
-    const int64_t tj = item / p.tiles_i;
-    const int i0 = (int)(item - tj * p.tiles_i) * T::TI, j0 = (int)tj * T::TJ;
+    int64_t ti, tj;
+    tile_of(blockIdx.x, p.tiles_i, p.tiles_j, ti, tj);
+    const int i0 = (int)ti * T::TI, j0 = (int)tj * T::TJ;
     const int e = blockIdx.y, z = blockIdx.z;
     const int64_t a = group_clamp(p.off[e], 0, p.total), b = group_clamp(p.off[e + 1], a, p.total);
     const int64_t per = ((b - a + p.splits - 1) / p.splits + T::KS - 1) / T::KS * T::KS;
@@ -120,22 +152,16 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_group_dw(GroupArgs p) {
             if (lane < 32 && j < p.N) db[j] = s;
         }
     }
-    if (split) {
-        float *o = p.part + ((int64_t)z * p.E + e) * p.N * p.K;
-        T::each(acc, [&](int i, int j, const auto &v) {
-            if (j0 + j >= p.N || i0 + i >= p.K) return;
-            const float f[4] = {v[0], v[1], v[2], v[3]};
-            store4<float>(o + (int64_t)(j0 + j) * p.K + i0 + i, f, p.K - i0 - i, p.K % 4 == 0);
-        });
-    } else {
-        O *o = reinterpret_cast<O *>(p.y) + (int64_t)e * p.N * p.K;
-        const bool aligned = p.K % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % (4 * sizeof(O)) == 0;
-        T::each(acc, [&](int i, int j, const auto &v) {
-            if (j0 + j >= p.N || i0 + i >= p.K) return;
-            const float f[4] = {v[0], v[1], v[2], v[3]};
-            store4<O>(o + (int64_t)(j0 + j) * p.K + i0 + i, f, p.K - i0 - i, aligned);
-        });
-    }
+    const auto out = [&](auto *o) {
+        typedef std::remove_reference_t<decltype(*o)> Out;
+        T::template write_out<RUN<Out>>(
+            smem, acc, [](int) { return 0; },
+            [&](int i, int j, const float (&v)[RUN<Out>], int) {
+                if (j0 + j < p.N && i0 + i < p.K) store_run<Out>(o + (int64_t)(j0 + j) * p.K + i0 + i, v, p.K - i0 - i);
+            });
+    };
+    if (split) out(p.part + ((int64_t)z * p.E + e) * p.N * p.K);
+    else out(reinterpret_cast<O *>(p.y) + (int64_t)e * p.N * p.K);
 }
 
 // The parts of dW and db, added in their order
@@ -165,16 +191,40 @@ static int group_check(srx_ctx *ctx, const char *name, int in_dtype, int out_dty
     return SRX_OK;
 }
 
-template <class El, class O, bool DX>
-static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
-    const int I = DX ? p.K : p.N;
-    typedef Tile<El, 2, 2, 2, 2, DX, false, false> T;
-    p.tiles_i = ceil_div64(I, T::TI);
+// Rows of an average group up to which the forward product is bound by reading W once
+static constexpr int64_t THIN_ROWS = 32;
+
+template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, bool DMA>
+static int group_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
+    typedef Tile<El, WI, WJ, FI, FJ, DX, false, DMA> T;
+    p.tiles_i = ceil_div64(DX ? p.K : p.N, T::TI);
     p.tiles_j = p.total / T::TJ + p.E;
     SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31), "%s: too many tiles", name);
     SrxProf prof_(ctx, DX ? "k_group_dx" : "k_group");
-    hipLaunchKernelGGL((k_group<El, O, DX, 2, 2, 2, 2, false>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
+    hipLaunchKernelGGL((k_group<El, O, DX, WI, WJ, FI, FJ, DMA>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
     return SRX_OK;
+}
+
+template <class El, class O, bool DX>
+static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
+    constexpr int Z = sizeof(El);
+    const int I = DX ? p.K : p.N;
+    if constexpr (!DX)
+        if (p.total <= THIN_ROWS * p.E) {
+            p.tiles_i = ceil_div64(p.N, 32);
+            p.tiles_j = p.total / 32 + p.E;
+            SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31), "%s: too many tiles", name);
+            SrxProf prof_(ctx, "k_group_thin");
+            hipLaunchKernelGGL((k_group_thin<El, O>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(THIN_WAVES * 64), 0, ctx->stream, p);
+            return SRX_OK;
+        }
+    if (I <= 64) return group_tile<El, O, DX, 1, 4, 2, 1, false>(ctx, name, p);
+    // W is read along its columns (extent K) by dx, along its rows (K) by the forward product
+    const bool dma = tile_dma(p.w, p.K, p.K, Z) && (DX ? tile_dma(p.dy, p.ld_dy, p.N, Z) : tile_dma(p.x, p.ld_x, p.K, Z));
+    if (!dma) return group_tile<El, O, DX, 2, 2, 2, 2, false>(ctx, name, p);
+    if (tile_large(ceil_div64(I, 256) * (p.total / 256 + (p.E + 1) / 2), ceil_div64(I, 128) * (p.total / 128 + (p.E + 1) / 2), ctx->num_cus))
+        return group_tile<El, O, DX, 4, 2, 2, 4, true>(ctx, name, p);
+    return group_tile<El, O, DX, 2, 2, 2, 2, true>(ctx, name, p);
 }
 
 template <bool DX>
@@ -220,43 +270,59 @@ extern "C" int srx_group_matmul_dx_dev(srx_ctx *ctx, int in_dtype, int out_dtype
     return group_types<true>(ctx, name, in_dtype, out_dtype, p);
 }
 
-// Parts that the rows of a group are cut into: enough tiles to fill the chip, and at least DW_MIN_ROWS rows of an average group
-// to a part
-static constexpr int64_t DW_TILES = 512, DW_MIN_ROWS = 512;
-static constexpr int DW_TILE = 128;
+// Tiles of dW, and the parts that the rows of a group are cut into where there are fewer tiles than fill the chip: the cheapest by
+// rounds of tiles (see tile_large), at least DW_MIN_ROWS rows of an average group to a part.  The sum of the parts costs about
+// DW_JOIN of a round of an average group's rows for each part's E N K.
+struct DwPlan { bool large; int splits; };
+static constexpr int64_t DW_MIN_ROWS = 512, DW_CUS = 256;
 
-static int group_splits(int E, int64_t total, int K, int N) {
-    const int64_t tiles = (int64_t)E * ceil_div64(K, DW_TILE) * ceil_div64(N, DW_TILE);
-    if (tiles == 0) return 1;
-    int64_t s = DW_TILES / tiles;
-    const int64_t most = total / E / DW_MIN_ROWS;
-    if (s > most) s = most;
-    return s < 1 ? 1 : s > 256 ? 256 : (int)s;
+static DwPlan group_dw_plan(int E, int64_t total, int K, int N) {
+    const int64_t nl = E * ceil_div64(K, 256) * ceil_div64(N, 256), ns = E * ceil_div64(K, 128) * ceil_div64(N, 128);
+    int64_t most = total / E / DW_MIN_ROWS;
+    most = most < 1 ? 1 : most > 64 ? 64 : most;
+    DwPlan best{false, 1};
+    double cost = 1e300;
+    // a round of whole groups of R rows, large tiles: about R * 28 ns (8,192 rows: 230 us); a part's write and read again at
+    // 4 TB/s
+    const double R = (double)total / E * 28e-9, part = 8.0 * E * N * (double)K / 4e12;
+    for (int64_t s = 1; s <= most; s++) {
+        const double join = s > 1 ? s * part + 4e-6 : 0.0;
+        const double l = (double)ceil_div64(nl * s, DW_CUS) * R / s + join, m = 0.63 * (double)ceil_div64(ns * s, 2 * DW_CUS) * R / s + join;
+        if (l < cost) { cost = l; best = {true, (int)s}; }
+        if (m < cost) { cost = m; best = {false, (int)s}; }
+    }
+    return best;
 }
 
 extern "C" int64_t srx_group_matmul_dw_scratch_bytes(const srx_ctx *ctx, int n_groups, int64_t total_rows, int K, int N) {
     if (!ctx || n_groups < 0 || n_groups > (1 << 20) || total_rows < 0 || total_rows > GROUP_MAX_ROWS || K < 1 || N < 1 || K > GROUP_MAX_DIM || N > GROUP_MAX_DIM) return -1;
     if (n_groups == 0) return 0;
-    const int64_t s = group_splits(n_groups, total_rows, K, N);
+    const int64_t s = group_dw_plan(n_groups, total_rows, K, N).splits;
     return s == 1 ? 0 : s * n_groups * N * ((int64_t)K + 1) * (int64_t)sizeof(float);
 }
 
-template <class El, class O>
-static int group_dw_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
-    typedef Tile<El, 2, 2, 2, 2, true, true, false> T;
+template <class El, class O, int WI, int WJ, int FI, int FJ, bool DMA>
+static int group_dw_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
+    typedef Tile<El, WI, WJ, FI, FJ, true, true, DMA> T;
     p.tiles_i = ceil_div64(p.K, T::TI);
     p.tiles_j = ceil_div64(p.N, T::TJ);
     SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31) && p.E <= 65535, "%s: too many tiles", name);
-    {
-        SrxProf prof_(ctx, "k_group_dw");
-        hipLaunchKernelGGL((k_group_dw<El, O, 2, 2, 2, 2, false>), dim3((unsigned)(p.tiles_i * p.tiles_j), (unsigned)p.E, (unsigned)p.splits), dim3(T::NT), 0, ctx->stream, p);
-    }
-    if (p.splits > 1) {
+    SrxProf prof_(ctx, "k_group_dw");
+    hipLaunchKernelGGL((k_group_dw<El, O, WI, WJ, FI, FJ, DMA>), dim3((unsigned)(p.tiles_i * p.tiles_j), (unsigned)p.E, (unsigned)p.splits), dim3(T::NT), 0, ctx->stream, p);
+    return SRX_OK;
+}
+
+template <class El, class O>
+static int group_dw_launch(srx_ctx *ctx, const char *name, GroupArgs &p, bool large) {
+    const bool dma = tile_dma(p.x, p.ld_x, p.K, sizeof(El)) && tile_dma(p.dy, p.ld_dy, p.N, sizeof(El));
+    const int rc = !dma ? group_dw_tile<El, O, 2, 2, 2, 2, false>(ctx, name, p)
+                 : large ? group_dw_tile<El, O, 2, 4, 4, 2, true>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, true>(ctx, name, p);
+    if (rc == SRX_OK && p.splits > 1) {
         const int64_t n = ceil_div64((int64_t)p.E * p.N * (p.K + 1ll), 256);
         SrxProf prof_(ctx, "k_group_join");
         hipLaunchKernelGGL((k_group_join<O>), dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, ctx->stream, p);
     }
-    return SRX_OK;
+    return rc;
 }
 
 extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *x_dev, int64_t ld_x,
@@ -273,16 +339,17 @@ extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype
     GroupArgs p{};
     p.dy = dy_dev; p.ld_dy = ld_dy; p.x = x_dev; p.ld_x = ld_x; p.y = dw_dev; p.dbias = dbias_dev;
     p.off = row_off_dev; p.total = total_rows; p.E = n_groups; p.K = K; p.N = N;
-    p.splits = group_splits(n_groups, total_rows, K, N);
+    const DwPlan plan = group_dw_plan(n_groups, total_rows, K, N);
+    p.splits = plan.splits;
     const int64_t need = srx_group_matmul_dw_scratch_bytes(ctx, n_groups, total_rows, K, N);
     if (need) {
         SRX_REQUIRE(ctx, scratch_dev && scratch_bytes >= need && srx_aligned(scratch_dev, 16), "%s: scratch of %lld bytes, %lld needed, 16-byte aligned (srx_group_matmul_dw_scratch_bytes)",
                     name, (long long)(scratch_dev ? scratch_bytes : 0), (long long)need);
         p.part = reinterpret_cast<float *>(scratch_dev);
     }
-    if (in_dtype == SRX_F32) rc = group_dw_launch<float, float>(ctx, name, p);
-    else if (in_dtype == SRX_F16) rc = out_dtype == SRX_F32 ? group_dw_launch<srx_f16, float>(ctx, name, p) : group_dw_launch<srx_f16, srx_f16>(ctx, name, p);
-    else rc = out_dtype == SRX_F32 ? group_dw_launch<srx_bf16, float>(ctx, name, p) : group_dw_launch<srx_bf16, srx_bf16>(ctx, name, p);
+    if (in_dtype == SRX_F32) rc = group_dw_launch<float, float>(ctx, name, p, plan.large);
+    else if (in_dtype == SRX_F16) rc = out_dtype == SRX_F32 ? group_dw_launch<srx_f16, float>(ctx, name, p, plan.large) : group_dw_launch<srx_f16, srx_f16>(ctx, name, p, plan.large);
+    else rc = out_dtype == SRX_F32 ? group_dw_launch<srx_bf16, float>(ctx, name, p, plan.large) : group_dw_launch<srx_bf16, srx_bf16>(ctx, name, p, plan.large);
     if (rc != SRX_OK) return rc;
     SRX_LAUNCH_CHECK(ctx);
     return SRX_OK;

@@ -62,27 +62,56 @@ template <class O, int WI, int WJ, int FI, int FJ>
 __global__ __launch_bounds__(WI *WJ * 64) void k_matmul_i8(I8Args p) {
     typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, true> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
-    const int64_t item = xcd_item(blockIdx.x, p.tiles_i * p.tiles_j);
-    const int64_t tj = item / p.tiles_i;
-    const int64_t i0 = (item - tj * p.tiles_i) * T::TI, j0 = tj * T::TJ;
+    int64_t i0, j0;
+    tile_of(blockIdx.x, p.tiles_i, p.tiles_j, i0, j0);
+    i0 *= T::TI;
+    j0 *= T::TJ;
     TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < T::TI ? p.I - i0 : T::TI)};
     TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < T::TJ ? p.J - j0 : T::TJ)};
     typename T::acc_t acc[FI][FJ];
     float none[FJ];
     T::template product<false>(smem, P, Q, (p.K + 15) / 16 * 16, acc, none, false);
     O *y = reinterpret_cast<O *>(p.y);
-    const bool aligned = (p.ld_y % 4 == 0) && (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(O)) == 0);
-    T::each(acc, [&](int i, int j, const auto &v) {
+    struct Held { float s[RUN<O>], b[RUN<O>]; };
+    T::template write_out<RUN<O>>(
+        smem, acc,
+        [&](int i) {
+            Held h;
+#pragma unroll
+            for (int e = 0; e < RUN<O>; e++) {
+                h.s[e] = i + e < P.n ? p.sp[i0 + i + e] : 0.0f;
+                h.b[e] = p.bias && p.bias_i && i + e < P.n ? p.bias[i0 + i + e] : 0.0f;
+            }
+            return h;
+        },
+        [&](int i, int j, const float (&v)[RUN<O>], const Held &h) {
+            if (j >= Q.n || i >= P.n) return;
+            const float sj = p.sq[j0 + j], bj = p.bias && !p.bias_i ? p.bias[j0 + j] : 0.0f;
+            float f[RUN<O>];
+#pragma unroll
+            for (int e = 0; e < RUN<O>; e++) f[e] = __builtin_fmaf(v[e] * sj, h.s[e], p.bias_i ? h.b[e] : bj);
+            store_run<O>(y + (j0 + j) * p.ld_y + i0 + i, f, P.n - i);
+        });
+}
+
+// Few rows: tiles of 32 x 32
+template <class O>
+__global__ __launch_bounds__(THIN_WAVES * 64) void k_matmul_i8_thin(I8Args p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[THIN_LDS];
+    const int64_t i0 = (blockIdx.x % p.tiles_i) * 32, j0 = (blockIdx.x / p.tiles_i) * 32;
+    const TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < 32 ? p.I - i0 : 32)};
+    const TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < 32 ? p.J - j0 : 32)};
+    O *y = reinterpret_cast<O *>(p.y);
+    thin_product<int8_t>(smem, P, Q, (p.K + 15) / 16 * 16, [&](int i, int j, const float (&v)[4]) {
         if (j >= Q.n || i >= P.n) return;
         const float sj = p.sq[j0 + j], bj = p.bias && !p.bias_i ? p.bias[j0 + j] : 0.0f;
         float f[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const bool in = i + e < P.n;
-            const float b = p.bias && p.bias_i ? (in ? p.bias[i0 + i + e] : 0.0f) : bj;
-            f[e] = __builtin_fmaf((float)v[e] * sj, in ? p.sp[i0 + i + e] : 0.0f, b);
+            f[e] = __builtin_fmaf(v[e] * sj, in ? p.sp[i0 + i + e] : 0.0f, p.bias && p.bias_i && in ? p.bias[i0 + i + e] : bj);
         }
-        store4<O>(y + (j0 + j) * p.ld_y + i0 + i, f, P.n - i, aligned);
+        store_four<O>(y + (j0 + j) * p.ld_y + i0 + i, f, P.n - i);
     });
 }
 
@@ -111,15 +140,32 @@ extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev,
     return SRX_OK;
 }
 
-template <class O>
-static int i8_launch(srx_ctx *ctx, const char *name, I8Args &p) {
-    typedef Tile<int8_t, 2, 2, 2, 2, false, false, true> T;
+// Rows up to which the product is bound by reading the weights once
+static constexpr int64_t I8_THIN_ROWS = 64;
+
+template <class O, int WI, int WJ, int FI, int FJ>
+static int i8_tile(srx_ctx *ctx, const char *name, I8Args &p) {
+    typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, true> T;
     p.tiles_i = ceil_div64(p.I, T::TI);
     p.tiles_j = ceil_div64(p.J, T::TJ);
     SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31), "%s: too many tiles", name);
     SrxProf prof_(ctx, "k_matmul_i8");
-    hipLaunchKernelGGL((k_matmul_i8<O, 2, 2, 2, 2>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
+    hipLaunchKernelGGL((k_matmul_i8<O, WI, WJ, FI, FJ>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
     return SRX_OK;
+}
+
+template <class O>
+static int i8_launch(srx_ctx *ctx, const char *name, I8Args &p, int64_t rows) {
+    if (rows <= I8_THIN_ROWS) {
+        p.tiles_i = ceil_div64(p.I, 32);
+        p.tiles_j = ceil_div64(p.J, 32);
+        SrxProf prof_(ctx, "k_matmul_i8_thin");
+        hipLaunchKernelGGL((k_matmul_i8_thin<O>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(THIN_WAVES * 64), 0, ctx->stream, p);
+        return SRX_OK;
+    }
+    if (tile_large(ceil_div64(p.I, 256) * ceil_div64(p.J, 256), ceil_div64(p.I, 128) * ceil_div64(p.J, 128), ctx->num_cus))
+        return i8_tile<O, 4, 2, 2, 4>(ctx, name, p);
+    return i8_tile<O, 2, 2, 2, 2>(ctx, name, p);
 }
 
 extern "C" int srx_matmul_i8_dev(srx_ctx *ctx, int out_dtype, const int8_t *xq_dev, int64_t ld_xq, const float *xs_dev, const int8_t *wq_dev, int64_t ld_wq,
@@ -150,7 +196,7 @@ extern "C" int srx_matmul_i8_dev(srx_ctx *ctx, int out_dtype, const int8_t *xq_d
         p.q = wq_dev; p.ld_q = ld_wq; p.sq = ws_dev; p.J = N;
         p.ld_y = stride_n;
     }
-    int rc = out_dtype == SRX_F32 ? i8_launch<float>(ctx, name, p) : out_dtype == SRX_F16 ? i8_launch<srx_f16>(ctx, name, p) : i8_launch<srx_bf16>(ctx, name, p);
+    int rc = out_dtype == SRX_F32 ? i8_launch<float>(ctx, name, p, rows) : out_dtype == SRX_F16 ? i8_launch<srx_f16>(ctx, name, p, rows) : i8_launch<srx_bf16>(ctx, name, p, rows);
     if (rc != SRX_OK) return rc;
     SRX_LAUNCH_CHECK(ctx);
     return SRX_OK;

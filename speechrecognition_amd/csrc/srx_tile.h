@@ -6,13 +6,13 @@
 // index adjacent ("columns": at base + k * ld + i), so that the three products of a linear layer -- x W^T, dy W and dy^T x --
 // read their operands where they lie.
 //
-// All types share one layout.  A slab is 128 bytes of reduction per row (64 16-bit, 32 f32, 128 8-bit elements), staged in LDS in
-// 16-byte chunks, double buffered; a k-step is 32 bytes: a lane's fragment is one chunk, its half-wave picks the chunk, which is
+// All types share one layout.  A slab is SLAB = 128 bytes of reduction per row (64 16-bit, 32 f32, 128 8-bit elements), staged in
+// LDS in 16-byte chunks, double buffered; a k-step is 32 bytes: a lane's fragment is one chunk, its half-wave picks the chunk, which is
 // the operand layout of v_mfma 32x32x16 (16 bit) and 32x32x32 (8 bit).  f32 runs four 32x32x2 on the chunk's four elements; any
 // order of k is right as long as both operands have the same.
 //
-// Rows slab: chunk c of row r at r * 128 + ((c ^ (r & 7)) << 4): the eight lanes that LDS serves together read eight different
-// bank groups.  Columns slab: [k][TX] with the column's 32-byte pairs moved by (k & 3): 16-bit fragments come through
+// Rows slab: chunk c of row r at r * 128 + ((c ^ (r & 7)) << 4): eight neighbouring rows' chunks lie on eight different bank
+// groups.  Columns slab: [k][TX] with the column's 32-byte pairs moved by (k & 3): 16-bit fragments come through
 // ds_read_b64_tr_b16 (each group of 16 lanes reads 4 k x 16 columns and gets them transposed), f32 ones element by element.
 //
 // Result layout: lane l holds column j = l & 31, rows 8 b + 4 (l >> 5) + 0..3 for b = 0..3: four adjacent i for one j.
@@ -63,15 +63,17 @@ struct TileOperand {
 
 typedef __attribute__((address_space(3))) unsigned char *lds_bytes;
 
-// All loads of the wave have landed, all its LDS reads are done, and so have everybody else's
+static constexpr int SLAB = 128, KSTEPS = SLAB / 32;
+
+// All loads of the wave have landed, all its LDS accesses are done, and so have everybody else's
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // COLS: the operand's layout (see above); TX its extent in the tile; NT threads
 template <class El, bool COLS, int TX, int NT>
 struct TileLoader {
-    static constexpr int Z = sizeof(El), EPC = 16 / Z, KS = 128 / Z;      // elements per chunk, per slab
-    static constexpr int CHUNKS = TX * 8, PER = CHUNKS / NT;
-    static constexpr int CPR = COLS ? TX * Z / 16 : 8;                    // chunks per slab row
+    static constexpr int Z = sizeof(El), EPC = 16 / Z, KS = SLAB / Z;     // elements per chunk, per slab
+    static constexpr int CHUNKS = TX * SLAB / 16, PER = CHUNKS / NT;
+    static constexpr int CPR = COLS ? TX * Z / 16 : SLAB / 16;            // chunks per slab row
     static_assert(CHUNKS % NT == 0 && (!COLS || CPR >= 8), "tile shape");
     static constexpr unsigned OUTSIDE = 0x80000000u;                      // past every bound: reads zeros
 
@@ -107,18 +109,17 @@ struct TileLoader {
     }
     // Straight into LDS, 16 bytes a lane, through a buffer descriptor whose bound makes everything outside the operand read
     // as zeros.  Host's condition: base and ld are whole chunks, so is the extent along a chunk (n or K); a slab's span < 2 GiB.
-    __device__ __forceinline__ void dma(int64_t k0, lds_bytes dst, int wave) const {
+    struct Slab { __amdgpu_buffer_rsrc_t r; int64_t left; unsigned at; };
+    __device__ __forceinline__ Slab slab(int64_t k0) const {
         const int64_t left = K - k0;
         const char *b = COLS ? base + k0 * ldb : base;
         const int64_t rows = COLS ? (left < KS ? left : KS) : n;
         const unsigned bound = rows > 0 ? (unsigned)((rows - 1) * ldb + (COLS ? (int64_t)n : K) * Z) : 0u;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(b), 0, bound, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            unsigned o = off[i];
-            if constexpr (!COLS) o = kin[i] < left ? o + (unsigned)(k0 * Z) : OUTSIDE;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(dst + (i * NT + wave * 64) * 16), 16, o, 0, 0, 0);
-        }
+        return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(b), 0, bound, 0x00020000), left, COLS ? 0u : (unsigned)(k0 * Z)};
+    }
+    __device__ __forceinline__ void dma(const Slab &s, int i, lds_bytes dst, int wave) const {
+        const unsigned o = COLS ? off[i] : kin[i] < s.left ? off[i] + s.at : OUTSIDE;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(s.r, (__attribute__((address_space(3))) void *)(dst + (i * NT + wave * 64) * 16), 16, o, 0, 0, 0);
     }
     // Any alignment and size: whole chunks by one (unaligned) 16-byte load, the rest element by element
     __device__ __forceinline__ void load(int64_t k0, i32x4_t (&v)[PER]) const {
@@ -147,12 +148,12 @@ struct TileLoader {
 // A lane's fragments of one operand, `first`: the wave's first row / column in the tile
 template <class El, bool COLS, int TX>
 struct TileReader {
-    unsigned at[4];
+    unsigned at[4];   // rows: by k-step; columns: by parity of the fragment (16 bit), by element (f32)
     __device__ __forceinline__ void init(int first, int lane) {
         const int h = lane >> 5;
         if constexpr (!COLS) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++) at[ks] = (first + (lane & 31)) * 128 + (((ks * 2 + h) ^ (lane & 7)) << 4);
+            for (int ks = 0; ks < KSTEPS; ks++) at[ks] = (first + (lane & 31)) * SLAB + (((ks * 2 + h) ^ (lane & 7)) << 4);
         } else if constexpr (sizeof(El) == 2) {
             const int q = lane & 15, k = q >> 2;
             const unsigned c = (first + ((lane >> 4) & 1) * 16 + (q & 3) * 4) * 2;
@@ -166,7 +167,7 @@ struct TileReader {
     __device__ __forceinline__ i32x4_t read(lds_bytes slab, int ks, int f) const {
         typedef __attribute__((address_space(3))) i32x4_t *vec_ptr;
         if constexpr (!COLS) {
-            return *reinterpret_cast<vec_ptr>(slab + at[ks] + f * 32 * 128);
+            return *reinterpret_cast<vec_ptr>(slab + at[ks] + f * 32 * SLAB);
         } else if constexpr (sizeof(El) == 2) {
             typedef __attribute__((address_space(3))) s16x4_t *half_ptr;
             const lds_bytes p = slab + at[f & 1] + (f >> 1) * 128 + ks * 16 * TX * 2;
@@ -187,14 +188,15 @@ template <class El, int WI_, int WJ_, int FI_, int FJ_, bool PC, bool QC, bool D
 struct Tile {
     static constexpr int WI = WI_, WJ = WJ_, FI = FI_, FJ = FJ_;
     static constexpr int NT = WI * WJ * 64, TI = WI * FI * 32, TJ = WJ * FJ * 32;
-    static constexpr int KS = 128 / sizeof(El);
-    static constexpr int STAGE = (TI + TJ) * 128, LDS = 2 * STAGE;
+    static constexpr int KS = SLAB / sizeof(El);
+    static constexpr int STAGE = (TI + TJ) * SLAB, LDS = 2 * STAGE;
     typedef typename MxType<El>::acc acc_t;
 
     // SUM: also sums[f] += sum over k of Q[j][k] for the lane's column of fragment f, its half-wave's part (sum_on: wanted)
     template <bool SUM>
     static __device__ __forceinline__ void product(unsigned char *smem, const TileOperand &P, const TileOperand &Q, int64_t K, acc_t (&acc)[FI][FJ],
                                                    float (&sums)[FJ], bool sum_on) {
+#if defined(__HIP_DEVICE_COMPILE__)   // (the compiler's host pass does not know all of the builtins)
         const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
         const int wi = wave % WI, wj = wave / WI;
         const lds_bytes lds = (lds_bytes)smem;
@@ -216,89 +218,267 @@ struct Tile {
         for (int j = 0; j < FJ; j++) sums[j] = 0.0f;
         const int64_t slabs = (K + KS - 1) / KS;
         if (slabs <= 0) return;
+        // Two slabs of LDS.  While slab s is multiplied, slab s + 1 is on its way (DMA: into the other half; otherwise: into
+        // registers).  Fragments are read one k-step ahead of their products; the barrier at a slab's end stands before its last
+        // k-step's products, when everything of the slab has been read, so that the next slab's first fragments and the loads of
+        // the slab after that one go out behind it.
+        constexpr int EACH = TileLoader<El, PC, TI, NT>::PER + TileLoader<El, QC, TJ, NT>::PER;
         i32x4_t vp[DMA ? 1 : lp.PER], vq[DMA ? 1 : lq.PER];
-        if constexpr (DMA) {
-            lp.dma(0, lds, wave);
-            lq.dma(0, lds + TI * 128, wave);
-        } else {
-            lp.load(0, vp);
-            lq.load(0, vq);
-            lp.store(vp, lds, t);
-            lq.store(vq, lds + TI * 128, t);
+        auto ahead = [&](int64_t s, int stage) __attribute__((always_inline)) {
+            const lds_bytes to = lds + stage * STAGE;
+            if constexpr (DMA) {
+                const auto sp = lp.slab(s * KS);
+                const auto sq = lq.slab(s * KS);
+#pragma unroll
+                for (int i = 0; i < lp.PER; i++) lp.dma(sp, i, to, wave);
+#pragma unroll
+                for (int i = 0; i < lq.PER; i++) lq.dma(sq, i, to + TI * SLAB, wave);
+            } else {
+                lp.load(s * KS, vp);
+                lq.load(s * KS, vq);
+            }
+        };
+        auto settle = [&](int stage) __attribute__((always_inline)) {   // registers into LDS
+            if constexpr (!DMA) {
+                const lds_bytes to = lds + stage * STAGE;
+                lp.store(vp, to, t);
+                lq.store(vq, to + TI * SLAB, t);
+            }
+        };
+        ahead(0, 0);
+        settle(0);
+        tile_barrier();
+        ahead(1, 1);
+        i32x4_t a[2][FI], b[2][FJ];
+        auto fetch = [&](int stage, int ks, int to) __attribute__((always_inline)) {
+            const lds_bytes from = lds + stage * STAGE;
+#pragma unroll
+            for (int i = 0; i < FI; i++) a[to][i] = rp.read(from, ks, i);
+#pragma unroll
+            for (int j = 0; j < FJ; j++) b[to][j] = rq.read(from + TI * SLAB, ks, j);
+        };
+        auto multiply = [&](int of, auto &&between) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < FI; i++)
+#pragma unroll
+                for (int j = 0; j < FJ; j++) {
+                    MxType<El>::mma(acc[i][j], a[of][i], b[of][j]);
+                    between(i * FJ + j);
+                }
+            if constexpr (SUM)
+                if (sum_on) {
+#pragma unroll
+                    for (int j = 0; j < FJ; j++) {
+                        El e[16 / sizeof(El)];
+                        __builtin_memcpy(e, &b[of][j], 16);
+#pragma unroll
+                        for (int q = 0; q < (int)(16 / sizeof(El)); q++) sums[j] += (float)e[q];
+                    }
+                }
+        };
+        fetch(0, 0, 0);
+        for (int64_t s = 0; s < slabs; s++) {
+            const int cur = s & 1, nxt = cur ^ 1;
+#pragma unroll
+            for (int ks = 0; ks + 1 < KSTEPS; ks++) {
+                fetch(cur, ks + 1, (ks + 1) & 1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(ks & 1, [](int) {});
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // (behind the last slab all this goes on with zeros, which nobody uses: one path for the accumulators)
+            settle(nxt);
+            tile_barrier();
+            fetch(nxt, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (DMA) {
+                // the new slab's loads go out between the products, whose pipe they leave alone
+                const lds_bytes to = lds + cur * STAGE;
+                const auto sp = lp.slab((s + 2) * KS);
+                const auto sq = lq.slab((s + 2) * KS);
+                multiply((KSTEPS - 1) & 1, [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < EACH; i++)
+                        if (i * (FI * FJ) / EACH == m) {
+                            if (i < lp.PER) lp.dma(sp, i < lp.PER ? i : 0, to, wave);
+                            else lq.dma(sq, i < lp.PER ? 0 : i - lp.PER, to + TI * SLAB, wave);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            } else {
+                ahead(s + 2, cur);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply((KSTEPS - 1) & 1, [](int) {});
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         tile_barrier();
-        for (int64_t s = 0; s < slabs; s++) {
-            const lds_bytes cur = lds + (s & 1) * STAGE, nxt = lds + ((s + 1) & 1) * STAGE;
-            const bool more = s + 1 < slabs;
-            if (more) {
-                if constexpr (DMA) {
-                    lp.dma((s + 1) * KS, nxt, wave);
-                    lq.dma((s + 1) * KS, nxt + TI * 128, wave);
-                } else {
-                    lp.load((s + 1) * KS, vp);
-                    lq.load((s + 1) * KS, vq);
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                i32x4_t a[FI], b[FJ];
-#pragma unroll
-                for (int i = 0; i < FI; i++) a[i] = rp.read(cur, ks, i);
-#pragma unroll
-                for (int j = 0; j < FJ; j++) b[j] = rq.read(cur + TI * 128, ks, j);
-#pragma unroll
-                for (int i = 0; i < FI; i++)
-#pragma unroll
-                    for (int j = 0; j < FJ; j++) MxType<El>::mma(acc[i][j], a[i], b[j]);
-                if constexpr (SUM)
-                    if (sum_on) {
-#pragma unroll
-                        for (int j = 0; j < FJ; j++) {
-                            El e[16 / sizeof(El)];
-                            __builtin_memcpy(e, &b[j], 16);
-#pragma unroll
-                            for (int q = 0; q < (int)(16 / sizeof(El)); q++) sums[j] += (float)e[q];
-                        }
-                    }
-            }
-            if constexpr (!DMA)
-                if (more) {
-                    lp.store(vp, nxt, t);
-                    lq.store(vq, nxt + TI * 128, t);
-                }
-            tile_barrier();
-        }
+#endif
     }
 
-    // f(i, j, v): v[0..3] are D[i .. i+3][j], i a multiple of 4, both counted within the tile
-    template <class F>
-    static __device__ __forceinline__ void each(const acc_t (&acc)[FI][FJ], F &&f) {
+    // Hands the tile out in runs of V adjacent i: emit(i, j, v, begin(i)) with v[0..V-1] = D[i .. i+V-1][j] in f32, i and j
+    // counted within the tile.  The accumulators' own order has four adjacent i per lane and a different j in every lane; each
+    // wave turns 32 of its columns at a time through its own part of LDS (free by now), so that the lanes of a row lie side by
+    // side: stores of whole lines (128 i of f32: 512 bytes) in place of 16-byte pieces.  A lane keeps its i for all rows.
+    template <int V, class Begin, class Emit>
+    static __device__ __forceinline__ void write_out(unsigned char *smem, const acc_t (&acc)[FI][FJ], Begin &&begin, Emit &&emit) {
+        constexpr int W = FI * 32, LPR = W / V, RPI = 64 / LPR;
+        static_assert(WI * WJ * W * 32 * 4 <= LDS && LPR <= 64, "tile shape");
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int i0 = (wave % WI) * FI * 32 + 4 * (lane >> 5), j0 = (wave / WI) * FJ * 32 + (lane & 31);
+        f32x4_t *st = reinterpret_cast<f32x4_t *>(smem + wave * (W * 32 * 4));
+        constexpr int MASK = (W / 4 < 32 ? W / 4 : 32) - 1;   // chunk c of row j at c ^ (j & MASK): no two lanes on one bank
+        const int h = lane >> 5, jw = lane & 31, ir = (lane % LPR) * V;
+        const auto held = begin((wave % WI) * W + ir);
 #pragma unroll
-        for (int j = 0; j < FJ; j++)
+        for (int f = 0; f < FJ; f++) {
 #pragma unroll
             for (int i = 0; i < FI; i++)
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    const decltype(acc[0][0][0] + acc[0][0][0]) v[4] = {acc[i][j][4 * b], acc[i][j][4 * b + 1], acc[i][j][4 * b + 2], acc[i][j][4 * b + 3]};
-                    f(i0 + i * 32 + b * 8, j0 + j * 32, v);
+                    const f32x4_t v = {(float)acc[i][f][4 * b], (float)acc[i][f][4 * b + 1], (float)acc[i][f][4 * b + 2], (float)acc[i][f][4 * b + 3]};
+                    st[jw * (W / 4) + ((i * 8 + b * 2 + h) ^ (jw & MASK))] = v;
                 }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = 0; r < 32 / RPI; r++) {
+                const int j = r * RPI + lane / LPR;
+                float v[V];
+#pragma unroll
+                for (int q = 0; q < V / 4; q++) {
+                    const f32x4_t x = st[j * (W / 4) + ((ir / 4 + q) ^ (j & MASK))];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[4 * q + e] = x[e];
+                }
+                emit((wave % WI) * W + ir, (wave / WI) * FJ * 32 + f * 32 + j, v, held);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 };
 
-// v[0..3] to p[0..3], the first `n` of them; whole and aligned quadruples as one store
+// Elements per 16-byte run of an output type
 template <class O>
-__device__ __forceinline__ void store4(O *p, const float (&v)[4], int64_t n, bool aligned) {
-    if (n >= 4 && aligned) *reinterpret_cast<typename SrxVec<O, 4>::type *>(p) = srx_pack<O, 4>(v);
+static constexpr int RUN = 16 / sizeof(O);
+
+// v to p[0 .. RUN), the first `n` of them; a whole run as one store, whatever its alignment
+template <class O>
+__device__ __forceinline__ void store_run(O *p, const float (&v)[RUN<O>], int64_t n) {
+    const typename SrxVec<O, RUN<O>>::type r = srx_pack<O, RUN<O>>(v);
+    if (n >= RUN<O>) __builtin_memcpy(p, &r, 16);
     else
-        for (int e = 0; e < 4; e++)
-            if (e < n) p[e] = srx_from_f32<O>(v[e]);
+#pragma unroll
+        for (int e = 0; e < RUN<O>; e++)
+            if (e < n) p[e] = r[e];
 }
 
-// Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its own: work item w of n for workgroup b, such that an
-// XCD works on a run of neighbouring items (which share their operands)
-__device__ __forceinline__ int64_t xcd_item(int64_t b, int64_t n) {
-    const int64_t q = n / 8, r = n % 8, x = b % 8, i = b / 8;
-    return x * q + (x < r ? x : r) + i;
+// A tile of 32 x 32 for few rows, where the other operand is read once and nothing else costs: THIN_WAVES waves take the slabs in
+// turn, straight from memory into fragments (a wave's four k-steps use whole lines), two slabs in flight each, and add their
+// parts through LDS.  Any alignment and size, rows layout for both operands.  emit(i, j, v): four adjacent i.
+static constexpr int THIN_WAVES = 8, THIN_LDS = THIN_WAVES * 32 * 32 * 4;
+
+template <class El>
+struct ThinOperand {
+    static constexpr int Z = sizeof(El), EPC = 16 / Z, KS = SLAB / Z;
+    const El *row;
+    bool live;
+    int64_t K;
+    __device__ __forceinline__ void init(const TileOperand &o, int64_t K_, int lane) {
+        live = (lane & 31) < o.n;
+        row = reinterpret_cast<const El *>(o.base) + (int64_t)(lane & 31) * o.ld + (lane >> 5) * EPC;
+        K = K_ - (lane >> 5) * EPC;   // elements from `row` on
+    }
+    __device__ __forceinline__ void load(int64_t slab, i32x4_t (&v)[KSTEPS]) const {
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ks++) {
+            const int64_t k = slab * KS + ks * 2 * EPC, have = live ? K - k : 0;
+            i32x4_t r = {0, 0, 0, 0};
+            if (have >= EPC) __builtin_memcpy(&r, row + k, 16);
+            else if (have > 0) {
+                El e[EPC];
+#pragma unroll
+                for (int q = 0; q < EPC; q++) e[q] = q < have ? row[k + q] : (El)0;
+                __builtin_memcpy(&r, e, 16);
+            }
+            v[ks] = r;
+        }
+    }
+};
+
+template <class El, class Emit>
+__device__ __forceinline__ void thin_product(unsigned char *smem, const TileOperand &P, const TileOperand &Q, int64_t K, Emit &&emit) {
+    typedef typename MxType<El>::acc acc_t;
+    typedef decltype(acc_t{}[0] + acc_t{}[0]) val;
+    typedef val val4 __attribute__((ext_vector_type(4)));
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    ThinOperand<El> p, q;
+    p.init(P, K, lane);
+    q.init(Q, K, lane);
+    acc_t acc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0;
+    const int64_t slabs = (K + p.KS - 1) / p.KS;
+    i32x4_t a[2][KSTEPS], b[2][KSTEPS];
+    p.load(wave, a[0]);
+    q.load(wave, b[0]);
+    for (int64_t s = wave; s < slabs; s += 2 * THIN_WAVES) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {   // (slabs past the end are zeros)
+            p.load(s + (u + 1) * THIN_WAVES, a[u ^ 1]);
+            q.load(s + (u + 1) * THIN_WAVES, b[u ^ 1]);
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ks++) MxType<El>::mma(acc, a[u][ks], b[u][ks]);
+        }
+    }
+    val4 *st = reinterpret_cast<val4 *>(smem);   // [wave][j][8 chunks of i, turned by j]
+    const int h = lane >> 5, j = lane & 31;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const val4 v = {acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]};
+        st[(wave * 32 + j) * 8 + ((2 * c + h) ^ (j & 7))] = v;
+    }
+    __syncthreads();
+    if (t < 256) {
+        const int oj = t >> 3, c = t & 7;
+        val4 v = st[oj * 8 + (c ^ (oj & 7))];
+#pragma unroll
+        for (int w = 1; w < THIN_WAVES; w++) v += st[(w * 32 + oj) * 8 + (c ^ (oj & 7))];
+        const float f[4] = {(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+        emit(c * 4, oj, f);
+    }
+}
+
+// v to p[0 .. 4), the first `n` of them
+template <class O>
+__device__ __forceinline__ void store_four(O *p, const float (&v)[4], int64_t n) {
+    const typename SrxVec<O, 4>::type r = srx_pack<O, 4>(v);
+    if (n >= 4) __builtin_memcpy(p, &r, 4 * sizeof(O));
+    else
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < n) p[e] = r[e];
+}
+
+// The tile (i, j) of workgroup b.  Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its own: an XCD gets a run
+// of neighbouring tiles, and the run goes through bands of TILE_BAND tiles of j, j first, so that the 32 tiles that its CUs hold at
+// a time are about 4 x 8 and read 12 operand slabs between them (in rows of i: 2 x 16 and 18).
+static constexpr int TILE_BAND = 8;
+__device__ __forceinline__ void tile_of(int64_t b, int64_t ni, int64_t nj, int64_t &i, int64_t &j) {
+    const int64_t n = ni * nj, q = n / 8, r = n % 8, x = b % 8;
+    const int64_t item = x * q + (x < r ? x : r) + b / 8;
+    const int64_t band = item / (TILE_BAND * ni), in = item - band * (TILE_BAND * ni);
+    const int64_t h = nj - band * TILE_BAND < TILE_BAND ? nj - band * TILE_BAND : TILE_BAND;
+    i = in / h;
+    j = band * TILE_BAND + (in - i * h);
+}
+
+// Tile of 256 x 256 on 8 waves or of 128 x 128 on 4?  A CU holds one of the former or two of the latter.  A round of the small
+// ones costs 0.63 of a round of the large (8 groups, 65,536 rows, 1,024 x 1,024 bf16: 20.8 us and 33 us; 165 us against 187 us in
+// all); few tiles are better spread over the chip as small ones.
+static inline bool tile_large(int64_t large, int64_t small, int64_t cus) {
+    return ceil_div64(large, cus) * 100 <= ceil_div64(small, 2 * cus) * 63;
+}
+// Can an operand's memory go straight into LDS (TileLoader::dma)?
+static inline bool tile_dma(const void *base, int64_t ld, int64_t extent, int z) {
+    const int64_t epc = 16 / z;
+    return srx_aligned(base, 16) && ld % epc == 0 && extent % epc == 0 && ld * z < (1 << 22);
 }

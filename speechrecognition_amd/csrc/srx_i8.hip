@@ -4,6 +4,8 @@
 //   y_rn = s_r s_n sum_k q_rk q_nk + b_n
 //
 // The sum is exact in 32 bits (K <= SRX_I8_MAX_K), so the only roundings are the scale's, the codes' and the output's few.
+#include <type_traits>
+
 #include "srx_tile.h"
 
 struct QuantArgs {
@@ -14,35 +16,114 @@ struct QuantArgs {
     float *scale;
 };
 
-// One wave per row: the maximum in a first sweep, the codes in a second that finds the row in cache.  HBM-bound.
+// A code is x / s rounded to a whole number, ties to even.  x times the hardware's reciprocal of s lies within 127 * 2^-22 = 3e-5
+// of the f32 quotient, so both round alike unless the product is nearly a half: only a run that holds such a value (one code in
+// 5,000) forms the quotients.  A division costs about ten instructions, and there is one per element.
+__device__ __forceinline__ int code_exact(float x, float s) {
+    const float c = rintf(x / s);
+    return (int)(c > 127.0f ? 127.0f : c < -127.0f ? -127.0f : c);   // (only a scale below the normal range can leave the range)
+}
+
+// |x| as a whole number that orders as it does, NaN above infinity above all others; two of a 16-bit type at a time
 template <class T>
-__global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs p) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (row >= p.rows) return;
-    const int lane = threadIdx.x & 63;
-    const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x;
-    float m = 0.0f;
-    for (int k = lane; k < p.K; k += 64) {
-        const float v = fabsf(srx_to_f32<T>(x[k]));
-        m = v > m || v != v ? v : m;   // a NaN stays
-    }
+struct Magnitude {
+    static constexpr int N = 16 / 4;
+    typedef uint16_t two __attribute__((ext_vector_type(2)));
+    typedef std::conditional_t<sizeof(T) == 4, uint32_t, two> part;
+    part m;
+    __device__ __forceinline__ void start() { m = {}; }
+    template <class R>
+    __device__ __forceinline__ void take(const R &run) {
+        part p[N];
+        __builtin_memcpy(p, &run, 16);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float v = __shfl_xor(m, o);
-        m = v > m || v != v ? v : m;
-    }
-    const float s = m / 127.0f;
-    if (lane == 0) p.scale[row] = s;
-    const bool live = s > 0.0f && s < __builtin_huge_valf();
-    int8_t *q = p.q + row * p.ld_q;
-    const int end = (p.K + 15) / 16 * 16;   // zeros up to whole 16 bytes: the product reads them
-    for (int k = lane; k < end; k += 64) {
-        int c = 0;
-        if (live && k < p.K) {
-            const float r = rintf(srx_to_f32<T>(x[k]) / s);
-            c = (int)(r > 127.0f ? 127.0f : r < -127.0f ? -127.0f : r);
+        for (int i = 0; i < N; i++) {
+            if constexpr (sizeof(T) == 4) m = max(m, p[i] & 0x7fffffffu);
+            else m = __builtin_elementwise_max(m, p[i] & (uint16_t)0x7fff);
         }
-        q[k] = (int8_t)c;
+    }
+    __device__ __forceinline__ float of_wave() const {   // the largest of all lanes
+        uint32_t v;
+        if constexpr (sizeof(T) == 4) v = m; else v = m.x > m.y ? m.x : m.y;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, v);
+        else return srx_to_f32<T>(__builtin_bit_cast(T, (uint16_t)v));
+    }
+};
+
+// A wave takes R rows, each in NV runs of 16 bytes per lane, and reads them once; NV = 0: one row of any length, its maximum in a
+// first sweep and the codes in a second.  HBM-bound: 3 bytes per element of a 16-bit type; several short rows per wave because
+// one row's loads (2 KB at 1,024 columns) do not cover their latency.
+template <class T, int NV, int R>
+__global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs p) {
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * R;
+    if (row0 >= p.rows) return;
+    const int lane = threadIdx.x & 63;
+    constexpr int V = RUN<T>;
+    const int end = (p.K + 15) / 16 * 16;   // zeros up to whole 16 bytes: the product reads them
+    typedef typename SrxVec<T, V>::type run;
+    auto load = [&](int64_t row, int k) {
+        const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x;
+        run v;
+        if (k + V <= p.K) __builtin_memcpy(&v, x + k, 16);
+        else
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = k + e < p.K ? x[k + e] : (T)0;
+        return v;
+    };
+    struct Scale { float s, rs; bool live, fast; };
+    auto scale = [&](int64_t row, float m) {
+        const float s = m / 127.0f;
+        if (lane == 0) p.scale[row] = s;
+        const float rs = __builtin_amdgcn_rcpf(s);   // infinite for a subnormal s: its codes all take the division
+        return Scale{s, rs, s > 0.0f && s < __builtin_huge_valf(), rs < __builtin_huge_valf()};
+    };
+    auto store = [&](int64_t row, int k, const run &v, const Scale &f) {
+        if (k >= end) return;
+        constexpr float whole = 12582912.0f;   // 3 * 2^22: added, it leaves the nearest whole number in the low bits
+        uint32_t c[V];
+        float off = 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float x = srx_to_f32<T>(v[e]), t = __builtin_fmaf(x, f.rs, whole);
+            off = fmaxf(off, fabsf(__builtin_fmaf(x, f.rs, whole - t)));
+            c[e] = __builtin_bit_cast(uint32_t, t);
+        }
+        if (!f.live || !f.fast || off > 0.4999f) {
+#pragma unroll
+            for (int e = 0; e < V; e++) c[e] = f.live ? (uint32_t)code_exact(srx_to_f32<T>(v[e]), f.s) : 0u;
+        }
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int e = 0; e < V / 4; e++)
+            w[e] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * e + 3], c[4 * e + 2], 0x0c0c0400u),
+                                         __builtin_amdgcn_perm(c[4 * e + 1], c[4 * e], 0x0c0c0400u), 0x05040100u);
+        __builtin_memcpy(p.q + row * p.ld_q + k, w, V);   // (end is a multiple of V)
+    };
+    if constexpr (NV > 0) {
+        run held[R][NV];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < NV; i++) held[r][i] = load(row0 + r < p.rows ? row0 + r : p.rows - 1, (i * 64 + lane) * V);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (row0 + r >= p.rows) return;
+            Magnitude<T> m;
+            m.start();
+#pragma unroll
+            for (int i = 0; i < NV; i++) m.take(held[r][i]);
+            const Scale f = scale(row0 + r, m.of_wave());
+#pragma unroll
+            for (int i = 0; i < NV; i++) store(row0 + r, (i * 64 + lane) * V, held[r][i], f);
+        }
+    } else {
+        Magnitude<T> m;
+        m.start();
+        for (int k = lane * V; k < p.K; k += 64 * V) m.take(load(row0, k));
+        const Scale f = scale(row0, m.of_wave());
+        for (int k = lane * V; k < end; k += 64 * V) store(row0, k, load(row0, k), f);
     }
 }
 
@@ -118,6 +199,24 @@ __global__ __launch_bounds__(THIN_WAVES * 64) void k_matmul_i8_thin(I8Args p) {
 // ------------------------------------------------------------------------------------------------ host side
 static constexpr int64_t I8_MAX_ROWS = 1ll << 40;
 
+// Several rows to a wave from this many rows on: fewer are better spread over the chip, one to a wave
+static constexpr int64_t QUANT_MANY = 16384;
+
+template <class T, int NV, int R>
+static void quant_rows(srx_ctx *ctx, const QuantArgs &p) {
+    hipLaunchKernelGGL((k_quantize_rows<T, NV, R>), dim3((unsigned)ceil_div64(p.rows, 4 * R)), dim3(256), 0, ctx->stream, p);
+}
+template <class T>
+static void quant_launch(srx_ctx *ctx, const QuantArgs &p) {
+    const int runs = (int)ceil_div64(p.K, 64 * RUN<T>);
+    const bool many = p.rows >= QUANT_MANY;
+    if (runs == 1) { if (many) quant_rows<T, 1, 8>(ctx, p); else quant_rows<T, 1, 1>(ctx, p); }
+    else if (runs == 2) { if (many) quant_rows<T, 2, 4>(ctx, p); else quant_rows<T, 2, 1>(ctx, p); }
+    else if (runs <= 4) { if (many) quant_rows<T, 4, 2>(ctx, p); else quant_rows<T, 4, 1>(ctx, p); }
+    else if (runs <= 8) quant_rows<T, 8, 1>(ctx, p);
+    else quant_rows<T, 0, 1>(ctx, p);
+}
+
 extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev, int64_t ld_x, int64_t rows, int K, int8_t *q_dev, int64_t ld_q, float *scale_dev) {
     const char *name = "srx_quantize_rows_dev";
     SRX_ENTER(ctx, name);
@@ -129,12 +228,11 @@ extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev,
                 "%s: row strides %lld / %lld for %d columns (codes: whole 16 bytes, 16-byte aligned)", name, (long long)ld_x, (long long)ld_q, K);
     SRX_REQUIRE(ctx, srx_aligned(x_dev, srx_dtype_size(dtype)) && srx_aligned(scale_dev, 4), "%s: misaligned buffer", name);
     const QuantArgs p{x_dev, ld_x, rows, ld_q, K, q_dev, scale_dev};
-    const dim3 g((unsigned)ceil_div64(rows, 4)), b(256);
     {
         SrxProf prof_(ctx, "k_quantize_rows");
-        if (dtype == SRX_F32) hipLaunchKernelGGL(k_quantize_rows<float>, g, b, 0, ctx->stream, p);
-        else if (dtype == SRX_F16) hipLaunchKernelGGL(k_quantize_rows<srx_f16>, g, b, 0, ctx->stream, p);
-        else hipLaunchKernelGGL(k_quantize_rows<srx_bf16>, g, b, 0, ctx->stream, p);
+        if (dtype == SRX_F32) quant_launch<float>(ctx, p);
+        else if (dtype == SRX_F16) quant_launch<srx_f16>(ctx, p);
+        else quant_launch<srx_bf16>(ctx, p);
     }
     SRX_LAUNCH_CHECK(ctx);
     return SRX_OK;

@@ -81,20 +81,18 @@ __device__ __forceinline__ void gate_of(float g, float &a, float &na) {
         a = g;
         na = 1.0f;
     } else {
-        // e = exp(-|g|) <= 1: a and 1 - a both come without cancellation.  16-bit types: the hardware's exp2 and reciprocal
-        // (a few 1e-7 relative, 1/1000 of the output's rounding); f32: the accurate functions.
-        float e, r;
+        // a = 1 / (1 + e), 1 - a = e a with e = exp(-g): both without cancellation.  The exponent is held at 115 (where a is
+        // 2^-115 and 1 - a is 1) so that e stays finite; a NaN passes.  16-bit types: the hardware's exp2 and reciprocal (a few
+        // 1e-7 relative, 1/1000 of the output's rounding); f32: the accurate functions.
         if constexpr (sizeof(T) == 4) {
-            e = expf(-fabsf(g));
-            r = 1.0f / (1.0f + e);
+            const float e = expf(g < -80.0f ? 80.0f : -g);
+            a = 1.0f / (1.0f + e);
+            na = e * a;
         } else {
-            e = __builtin_amdgcn_exp2f(-1.44269504088896340736f * fabsf(g));
-            r = __builtin_amdgcn_rcpf(1.0f + e);
+            const float t = -1.44269504088896340736f * g, e = __builtin_amdgcn_exp2f(t > 115.0f ? 115.0f : t);
+            a = __builtin_amdgcn_rcpf(1.0f + e);
+            na = e * a;
         }
-        const float er = e * r;
-        a = g >= 0.0f ? r : er;
-        na = g >= 0.0f ? er : r;
-        if (g != g) a = na = g;
     }
 }
 
@@ -121,22 +119,35 @@ __device__ __forceinline__ bool lane_item(const ScanArgs &p, int64_t nseg, int64
 template <class T, int V>
 struct Rows { typename SrxVec<T, V>::type r[SB]; };
 
-// SB rows from `row` on (rows behind end - 1 repeat it: in bounds, their values are not used)
+// SB rows from `row` on (rows behind end - 1 repeat it: in bounds, their values are not used).  The row's address is uniform where
+// the wave works on one segment, the lane adds its 32-bit offset: one scalar add per row
 template <class T, int V>
-__device__ __forceinline__ void load_rows(Rows<T, V> &d, const void *p, int64_t ld, int64_t row, int64_t end, int ch) {
+__device__ __forceinline__ void load_rows(Rows<T, V> &d, const void *p, int64_t ld, int64_t row, int64_t end, unsigned ch) {
     typedef typename SrxVec<T, V>::type vec;
-    const T *base = reinterpret_cast<const T *>(p);
+    const char *base = reinterpret_cast<const char *>(p) + row * ld * (int64_t)sizeof(T);
+    const int64_t step = ld * (int64_t)sizeof(T);
+    const unsigned lane = ch * (unsigned)sizeof(T);
+    if (row + SB <= end) {
 #pragma unroll
-    for (int i = 0; i < SB; i++) {
-        const int64_t r = row + i < end ? row + i : end - 1;
-        d.r[i] = *reinterpret_cast<const vec *>(base + r * ld + ch);
+        for (int i = 0; i < SB; i++) {
+            d.r[i] = *reinterpret_cast<const vec *>(base + lane);
+            base += step;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < SB; i++) {
+            d.r[i] = *reinterpret_cast<const vec *>(base + lane);
+            if (row + i + 1 < end) base += step;
+        }
     }
 }
 
 template <class T, int V>
-__device__ __forceinline__ void store_row(void *p, int64_t ld, int64_t row, int ch, const float (&f)[V]) {
-    *reinterpret_cast<typename SrxVec<T, V>::type *>(reinterpret_cast<T *>(p) + row * ld + ch) = srx_pack<T, V>(f);
+__device__ __forceinline__ void store_row(char *row, unsigned ch, const float (&f)[V]) {
+    *reinterpret_cast<typename SrxVec<T, V>::type *>(row + ch * (unsigned)sizeof(T)) = srx_pack<T, V>(f);
 }
+template <class T>
+__device__ __forceinline__ char *row_at(void *p, int64_t ld, int64_t row) { return reinterpret_cast<char *>(p) + row * ld * (int64_t)sizeof(T); }
 
 // ---- forward, main pass
 template <class T, int MODE, int V, bool UNI>
@@ -169,6 +180,7 @@ __global__ __launch_bounds__(256) void k_scan(ScanArgs p) {
                 keep += p.D;
             }
             const bool full = row + SB <= g.end;
+            char *out = row_at<T>(p.h, p.ld_h, row);
 #pragma unroll
             for (int i = 0; i < SB; i++) {
                 float a[V], b[V];
@@ -182,7 +194,8 @@ __global__ __launch_bounds__(256) void k_scan(ScanArgs p) {
                 if (full || row + i < g.end) {
 #pragma unroll
                     for (int v = 0; v < V; v++) st[v] = __builtin_fmaf(a[v], st[v], b[v]);
-                    store_row<T, V>(p.h, p.ld_h, row + i, ch, st);
+                    store_row<T, V>(out, ch, st);
+                    out += p.ld_h * (int64_t)sizeof(T);
                 }
             }
             ga = gn;
@@ -244,6 +257,7 @@ __global__ __launch_bounds__(256) void k_scan_back(ScanArgs p) {
                     sa[v] = __builtin_fmaf(av[i][v], sa[v], MODE == SRX_SCAN_VALUE ? xv : nav[i][v] * xv);
                 }
             }
+            char *odx = row_at<T>(p.dx, p.ld_dx, row), *odg = row_at<T>(p.dgate, p.ld_dgate, row);
 #pragma unroll
             for (int i = SB - 1; i >= 0; i--) {
                 if (full || row + i < g.end) {
@@ -260,8 +274,8 @@ __global__ __launch_bounds__(256) void k_scan_back(ScanArgs p) {
                         }
                         c[v] = av[i][v] * lam;
                     }
-                    store_row<T, V>(p.dx, p.ld_dx, row + i, ch, dx);
-                    store_row<T, V>(p.dgate, p.ld_dgate, row + i, ch, dg);
+                    store_row<T, V>(odx + i * (p.ld_dx * (int64_t)sizeof(T)), ch, dx);
+                    store_row<T, V>(odg + i * (p.ld_dgate * (int64_t)sizeof(T)), ch, dg);
                 }
             }
             ga = gn;

@@ -95,6 +95,25 @@ class DevArray:
         a.borrowed = True
         return a
 
+    # what the learned layers' calls ask of a buffer, under the names that a torch tensor has
+    def data_ptr(self):
+        return self.ptr.value
+
+    def stride(self):
+        return tuple(int(np.prod(self.shape[i + 1:], dtype=np.int64)) for i in range(len(self.shape)))
+
+    def numel(self):
+        return int(np.prod(self.shape, dtype=np.int64))
+
+    def element_size(self):
+        return self.dtype.itemsize
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return self.ctx.device
+
     def upload(self, host):
         host = np.ascontiguousarray(host, dtype=self.dtype)
         assert host.nbytes == self.nbytes, (host.shape, self.shape)
@@ -587,68 +606,57 @@ def gather_gid(ctx, hmm, path_d, status_d):
 # ----------------------------------------------------------------------------- learned layers
 # Device buffers of these calls are DevArrays (bf16 held as uint16) or torch tensors on the context's device.  The library's
 # calls are asynchronous on the context's stream: a tensor that another stream writes or reads is ordered by the caller.
+# A serving step's call is launch-bound, so the checks below are written for few interpreter steps.
 SCAN_VALUE, SCAN_SIGMOID = _capi.SRX_SCAN_VALUE, _capi.SRX_SCAN_SIGMOID
-_DTYPES = {"float32": _capi.SRX_F32, "float16": _capi.SRX_F16, "uint16": _capi.SRX_BF16, "bfloat16": _capi.SRX_BF16, "int8": "i8",
-           "int64": "i64", "uint8": "u8"}
+_I8, _I64 = 16, 17
+_DTYPES = {}
+_DTYPE_NAMES = {"float32": _capi.SRX_F32, "float16": _capi.SRX_F16, "uint16": _capi.SRX_BF16, "bfloat16": _capi.SRX_BF16, "int8": _I8, "int64": _I64}
 
 
 def _typed(a):
-    """Element type of a DevArray or a torch tensor: SRX_F32 / SRX_F16 / SRX_BF16, or "i8" / "i64" / "u8"."""
-    t = _DTYPES.get(a.dtype)
-    if t is None:
-        t = _DTYPES.get(str(a.dtype).replace("torch.", ""))
-        if t is None:
-            raise ValueError(f"element type {a.dtype} is not supported")
-        _DTYPES[a.dtype] = t
-    return t
+    """Element type of a DevArray or a torch tensor: SRX_F32 / SRX_F16 / SRX_BF16, or _I8 / _I64 (-1: none of them)."""
+    try:
+        return _DTYPES[a.dtype]
+    except KeyError:
+        t = _DTYPES[a.dtype] = _DTYPE_NAMES.get(str(a.dtype).replace("torch.", ""), -1)
+        return t
 
 
-def _buf(a, ctx):
-    """Device address of a DevArray or a torch tensor (None: null)."""
+def _refuse(what, a, wanted):
+    where = f" on device {a.get_device()}" if hasattr(a, "get_device") else ""
+    raise ValueError(f"{what}: {tuple(a.shape)} {a.dtype}{where}, strides {tuple(a.stride())}; wanted {wanted}")
+
+
+def _rows(a, shape, t, what, dev):
+    """(address, row stride) of a matrix with adjacent columns."""
+    st = a.stride()
+    if a.shape != shape or _typed(a) != t or a.get_device() != dev or (st[1] != 1 and shape[1] > 1) or (st[0] < shape[1] and shape[0] > 1):
+        _refuse(what, a, f"{tuple(shape)} of the call's element type with adjacent columns on device {dev}")
+    return a.data_ptr(), st[0] if st[0] > shape[1] else shape[1]
+
+
+def _dense(a, n, t, what, dev):
+    """Address of `n` contiguous elements (None: null)."""
     if a is None:
         return None
-    if hasattr(a, "data_ptr"):
-        if a.device.type != "cuda" or a.device.index != ctx.device:
-            raise ValueError(f"a tensor on {a.device}: the context works on device {ctx.device}")
-        return a.data_ptr()
-    return a.ptr
+    if a.numel() != n or _typed(a) != t or a.get_device() != dev or not a.is_contiguous():
+        _refuse(what, a, f"{n} contiguous elements of the call's type on device {dev}")
+    return a.data_ptr()
 
 
-def _strides(a):
-    if hasattr(a, "data_ptr"):
-        return a.stride()
-    s, r = [], 1
-    for n in reversed(a.shape):
-        s.append(r)
-        r *= n
-    return tuple(reversed(s))
-
-
-def _rows(a, rows, cols, dtype, what, ctx):
-    """(address, row stride) of a [rows][cols] matrix with adjacent columns."""
-    st = _strides(a)
-    if tuple(a.shape) != (rows, cols) or _typed(a) != dtype or (cols > 1 and st[1] != 1) or (rows > 1 and st[0] < cols):
-        raise ValueError(f"{what}: {tuple(a.shape)} {a.dtype} with strides {tuple(st)}, wanted [{rows}][{cols}] of one type with adjacent columns")
-    return _buf(a, ctx), max(st[0], cols)
-
-
-def _dense(a, shape, dtype, what, ctx):
-    """Address of a contiguous array of that shape and type, or of one with as many elements in a single dimension."""
-    if a is None:
-        return None
-    n = 1
-    for v in shape:
-        n *= v
-    if (tuple(a.shape) != tuple(shape) and tuple(a.shape) != (n,)) or _typed(a) != dtype or (hasattr(a, "data_ptr") and not a.is_contiguous()):
-        raise ValueError(f"{what}: {tuple(a.shape)} {a.dtype}, wanted contiguous {tuple(shape)}")
-    return _buf(a, ctx)
-
-
-def _room(a, ctx):
+def _room(a, what, dev):
     """(address, bytes) of a caller's scratch or state buffer."""
     if a is None:
         return None, 0
-    return _buf(a, ctx), a.nbytes if isinstance(a, DevArray) else a.numel() * a.element_size()
+    if a.get_device() != dev or not a.is_contiguous():
+        _refuse(what, a, f"contiguous memory on device {dev}")
+    return a.data_ptr(), a.numel() * a.element_size()
+
+
+def _one_of(t, what, a):
+    if t > _capi.SRX_BF16 or t < 0:
+        _refuse(what, a, "f32, f16 or bf16 (uint16)")
+    return t
 
 
 def gated_scan_scratch_bytes(ctx, n_utt, total_frames, max_frames, D):
@@ -662,68 +670,77 @@ def gated_scan_states_bytes(ctx, n_utt, total_frames, D):
 def gated_scan(ctx, mode, gate, x, frame_off, max_frames, h, h0=None, h_last=None, states=None, scratch=None):
     """h_t = a_t h_(t-1) + x_t (SCAN_VALUE, a = gate) or a_t h_(t-1) + (1 - a_t) x_t (SCAN_SIGMOID, a = sigmoid(gate)) along every
     utterance: gate, x -> h [T][D]; h0 -> h_last [n_utt][D] f32.  states (gated_scan_states_bytes): for gated_scan_backward."""
-    T, D = x.shape
-    n, t = frame_off.shape[0] - 1, _typed(x)
-    g, ldg = _rows(gate, T, D, t, "gate", ctx)
-    xp, ldx = _rows(x, T, D, t, "x", ctx)
-    hp, ldh = _rows(h, T, D, t, "h", ctx)
-    sp, sn = _room(states, ctx)
+    shape, dev = x.shape, ctx.device
+    T, D = shape
+    n, t = frame_off.numel() - 1, _one_of(_typed(x), "x", x)
+    g, ldg = _rows(gate, shape, t, "gate", dev)
+    xp, ldx = _rows(x, shape, t, "x", dev)
+    hp, ldh = _rows(h, shape, t, "h", dev)
+    sp, sn = _room(states, "states", dev)
     if states is not None and sn < gated_scan_states_bytes(ctx, n, T, D):
         raise ValueError(f"states: {sn} bytes, {gated_scan_states_bytes(ctx, n, T, D)} needed")
-    wp, wn = _room(scratch, ctx)
-    check(ctx.lib.srx_gated_scan_dev(ctx.h, mode, t, g, ldg, xp, ldx, _dense(h0, (n, D), 0, "h0", ctx), _dense(frame_off, (n + 1,), "i64", "frame_off", ctx),
-                                     n, T, max_frames, D, hp, ldh, _dense(h_last, (n, D), 0, "h_last", ctx), sp, wp, wn), ctx.h)
+    wp, wn = _room(scratch, "scratch", dev)
+    rc = ctx.lib.srx_gated_scan_dev(ctx.h, mode, t, g, ldg, xp, ldx, _dense(h0, n * D, 0, "h0", dev), _dense(frame_off, n + 1, _I64, "frame_off", dev),
+                                    n, T, max_frames, D, hp, ldh, _dense(h_last, n * D, 0, "h_last", dev), sp, wp, wn)
+    if rc:
+        check(rc, ctx.h)
     return h
 
 
 def gated_scan_backward(ctx, mode, gate, x, frame_off, max_frames, states, dh, dgate, dx, dh_last=None, dh0=None, scratch=None):
     """Gradients of gated_scan: dh [T][D] (and dh_last [n_utt][D]) -> dgate, dx [T][D] (and dh0 [n_utt][D])."""
-    T, D = x.shape
-    n, t = frame_off.shape[0] - 1, _typed(x)
-    g, ldg = _rows(gate, T, D, t, "gate", ctx)
-    xp, ldx = _rows(x, T, D, t, "x", ctx)
-    dp, ldd = _rows(dh, T, D, t, "dh", ctx)
-    gp, ldgp = _rows(dgate, T, D, t, "dgate", ctx)
-    op, ldo = _rows(dx, T, D, t, "dx", ctx)
-    sp, sn = _room(states, ctx)
+    shape, dev = x.shape, ctx.device
+    T, D = shape
+    n, t = frame_off.numel() - 1, _one_of(_typed(x), "x", x)
+    g, ldg = _rows(gate, shape, t, "gate", dev)
+    xp, ldx = _rows(x, shape, t, "x", dev)
+    dp, ldd = _rows(dh, shape, t, "dh", dev)
+    gp, ldgp = _rows(dgate, shape, t, "dgate", dev)
+    op, ldo = _rows(dx, shape, t, "dx", dev)
+    sp, sn = _room(states, "states", dev)
     if sn < gated_scan_states_bytes(ctx, n, T, D):
         raise ValueError(f"states: {sn} bytes, {gated_scan_states_bytes(ctx, n, T, D)} needed")
-    wp, wn = _room(scratch, ctx)
-    check(ctx.lib.srx_gated_scan_backward_dev(ctx.h, mode, t, g, ldg, xp, ldx, sp, dp, ldd, _dense(dh_last, (n, D), 0, "dh_last", ctx),
-                                              _dense(frame_off, (n + 1,), "i64", "frame_off", ctx), n, T, max_frames, D, gp, ldgp, op, ldo,
-                                              _dense(dh0, (n, D), 0, "dh0", ctx), wp, wn), ctx.h)
+    wp, wn = _room(scratch, "scratch", dev)
+    rc = ctx.lib.srx_gated_scan_backward_dev(ctx.h, mode, t, g, ldg, xp, ldx, sp, dp, ldd, _dense(dh_last, n * D, 0, "dh_last", dev),
+                                             _dense(frame_off, n + 1, _I64, "frame_off", dev), n, T, max_frames, D, gp, ldgp, op, ldo,
+                                             _dense(dh0, n * D, 0, "dh0", dev), wp, wn)
+    if rc:
+        check(rc, ctx.h)
     return dgate, dx
 
 
-def _weights(w, n, dtype, what, ctx):
-    if len(w.shape) != 3 or w.shape[0] != n:
-        raise ValueError(f"{what}: {tuple(w.shape)}, wanted [{n}][outputs][inputs]")
-    return _dense(w, tuple(w.shape), dtype, what, ctx)
+def _weights(w, E, N, K, t, dev):
+    if w.shape != (E, N, K):
+        _refuse("w", w, f"[{E}][{N}][{K}]")
+    return _dense(w, E * N * K, t, "w", dev)
 
 
 def group_matmul(ctx, x, w, row_off, y, bias=None):
     """y_r = W_e x_r + b_e for the rows r of group e: x [T][K], w [E][N][K], bias [E][N] f32 -> y [T][N] (x's type or f32)."""
-    (T, K), E, t = x.shape, row_off.shape[0] - 1, _typed(x)
+    dev = ctx.device
+    T, K = x.shape
+    E, t, o = row_off.numel() - 1, _one_of(_typed(x), "x", x), _one_of(_typed(y), "y", y)
     N = w.shape[1]
-    xp, ldx = _rows(x, T, K, t, "x", ctx)
-    yp, ldy = _rows(y, T, N, _typed(y), "y", ctx)
-    if w.shape[2] != K:
-        raise ValueError(f"w: {tuple(w.shape)}, wanted [{E}][{N}][{K}]")
-    check(ctx.lib.srx_group_matmul_dev(ctx.h, t, _typed(y), xp, ldx, _weights(w, E, t, "w", ctx), _dense(bias, (E, N), 0, "bias", ctx),
-                                       _dense(row_off, (E + 1,), "i64", "row_off", ctx), E, T, K, N, yp, ldy), ctx.h)
+    xp, ldx = _rows(x, x.shape, t, "x", dev)
+    yp, ldy = _rows(y, (T, N), o, "y", dev)
+    rc = ctx.lib.srx_group_matmul_dev(ctx.h, t, o, xp, ldx, _weights(w, E, N, K, t, dev), _dense(bias, E * N, 0, "bias", dev),
+                                      _dense(row_off, E + 1, _I64, "row_off", dev), E, T, K, N, yp, ldy)
+    if rc:
+        check(rc, ctx.h)
     return y
 
 
 def group_matmul_dx(ctx, dy, w, row_off, dx):
     """dx_r = W_e^T dy_r: dy [T][N], w [E][N][K] -> dx [T][K] (dy's type or f32)."""
-    (T, N), E, t = dy.shape, row_off.shape[0] - 1, _typed(dy)
+    dev = ctx.device
+    T, N = dy.shape
+    E, t, o = row_off.numel() - 1, _one_of(_typed(dy), "dy", dy), _one_of(_typed(dx), "dx", dx)
     K = w.shape[2]
-    dp, ldd = _rows(dy, T, N, t, "dy", ctx)
-    op, ldo = _rows(dx, T, K, _typed(dx), "dx", ctx)
-    if w.shape[1] != N:
-        raise ValueError(f"w: {tuple(w.shape)}, wanted [{E}][{N}][{K}]")
-    check(ctx.lib.srx_group_matmul_dx_dev(ctx.h, t, _typed(dx), dp, ldd, _weights(w, E, t, "w", ctx), _dense(row_off, (E + 1,), "i64", "row_off", ctx),
-                                          E, T, K, N, op, ldo), ctx.h)
+    dp, ldd = _rows(dy, dy.shape, t, "dy", dev)
+    op, ldo = _rows(dx, (T, K), o, "dx", dev)
+    rc = ctx.lib.srx_group_matmul_dx_dev(ctx.h, t, o, dp, ldd, _weights(w, E, N, K, t, dev), _dense(row_off, E + 1, _I64, "row_off", dev), E, T, K, N, op, ldo)
+    if rc:
+        check(rc, ctx.h)
     return dx
 
 
@@ -733,43 +750,58 @@ def group_matmul_dw_scratch_bytes(ctx, n_groups, total_rows, K, N):
 
 def group_matmul_dw(ctx, dy, x, row_off, dw, dbias=None, scratch=None):
     """dW_e = sum of dy_r x_r^T, db_e = sum of dy_r over the rows of group e: dy [T][N], x [T][K] -> dw [E][N][K], dbias [E][N] f32."""
-    (T, N), E, t = dy.shape, row_off.shape[0] - 1, _typed(dy)
+    dev = ctx.device
+    T, N = dy.shape
+    E, t, o = row_off.numel() - 1, _one_of(_typed(dy), "dy", dy), _one_of(_typed(dw), "dw", dw)
     K = x.shape[1]
-    dp, ldd = _rows(dy, T, N, t, "dy", ctx)
-    xp, ldx = _rows(x, T, K, t, "x", ctx)
-    wp, wn = _room(scratch, ctx)
-    check(ctx.lib.srx_group_matmul_dw_dev(ctx.h, t, _typed(dw), dp, ldd, xp, ldx, _dense(row_off, (E + 1,), "i64", "row_off", ctx), E, T, K, N,
-                                          _dense(dw, (E, N, K), _typed(dw), "dw", ctx), _dense(dbias, (E, N), 0, "dbias", ctx), wp, wn), ctx.h)
+    dp, ldd = _rows(dy, dy.shape, t, "dy", dev)
+    xp, ldx = _rows(x, (T, K), t, "x", dev)
+    wp, wn = _room(scratch, "scratch", dev)
+    rc = ctx.lib.srx_group_matmul_dw_dev(ctx.h, t, o, dp, ldd, xp, ldx, _dense(row_off, E + 1, _I64, "row_off", dev), E, T, K, N,
+                                         _weights(dw, E, N, K, o, dev), _dense(dbias, E * N, 0, "dbias", dev), wp, wn)
+    if rc:
+        check(rc, ctx.h)
     return dw
 
 
 def quantize_rows(ctx, x, q, scale):
     """scale_r = max |x_r| / 127, q_r = round(x_r / scale_r): x [T][K] -> codes q [T][>= K, whole 16 bytes] int8, scale [T] f32."""
+    dev = ctx.device
     T, K = x.shape
-    xp, ldx = _rows(x, T, K, _typed(x), "x", ctx)
-    qp, ldq = _rows(q, T, q.shape[1], "i8", "q", ctx)
+    t = _one_of(_typed(x), "x", x)
+    xp, ldx = _rows(x, x.shape, t, "x", dev)
     if q.shape[1] < (K + 15) // 16 * 16:
-        raise ValueError(f"q: {tuple(q.shape)}, wanted [{T}][{(K + 15) // 16 * 16}]")
-    check(ctx.lib.srx_quantize_rows_dev(ctx.h, _typed(x), xp, ldx, T, K, qp, ldq, _dense(scale, (T,), 0, "scale", ctx)), ctx.h)
+        _refuse("q", q, f"[{T}][{(K + 15) // 16 * 16}]")
+    qp, ldq = _rows(q, (T, q.shape[1]), _I8, "q", dev)
+    rc = ctx.lib.srx_quantize_rows_dev(ctx.h, t, xp, ldx, T, K, qp, ldq, _dense(scale, T, 0, "scale", dev))
+    if rc:
+        check(rc, ctx.h)
     return q, scale
 
 
 def matmul_i8(ctx, xq, xs, wq, ws, K, y, bias=None):
     """y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n: codes xq [T][>= K], wq [N][>= K] int8, scales f32 -> y [T][N] (also a
     transposed view: scores state by state)."""
-    T, N = xq.shape[0], wq.shape[0]
-    k16 = (K + 15) // 16 * 16
-    xp, ldx = _rows(xq, T, xq.shape[1], "i8", "xq", ctx)
-    wp, ldw = _rows(wq, N, wq.shape[1], "i8", "wq", ctx)
-    if xq.shape[1] < k16 or wq.shape[1] < k16 or tuple(y.shape) != (T, N):
-        raise ValueError(f"codes {tuple(xq.shape)}, {tuple(wq.shape)}, scores {tuple(y.shape)} for K = {K}")
-    sr, sn = _strides(y)
+    dev = ctx.device
+    T, N, k16 = xq.shape[0], wq.shape[0], (K + 15) // 16 * 16
+    if xq.shape[1] < k16:
+        _refuse("xq", xq, f"rows of {k16} codes")
+    if wq.shape[1] < k16:
+        _refuse("wq", wq, f"rows of {k16} codes")
+    xp, ldx = _rows(xq, xq.shape, _I8, "xq", dev)
+    wp, ldw = _rows(wq, wq.shape, _I8, "wq", dev)
+    o = _one_of(_typed(y), "y", y)
+    if y.shape != (T, N) or y.get_device() != dev:
+        _refuse("y", y, f"[{T}][{N}] on device {dev}")
+    sr, sn = y.stride()
     if sn == 1 or N == 1:
         sr, sn = max(sr, N) if T == 1 else sr, 1
     elif T == 1:
         sr, sn = 1, max(sn, T)
-    check(ctx.lib.srx_matmul_i8_dev(ctx.h, _typed(y), xp, ldx, _dense(xs, (T,), 0, "xs", ctx), wp, ldw, _dense(ws, (N,), 0, "ws", ctx),
-                                    _dense(bias, (N,), 0, "bias", ctx), T, N, K, _buf(y, ctx), sr, sn), ctx.h)
+    rc = ctx.lib.srx_matmul_i8_dev(ctx.h, o, xp, ldx, _dense(xs, T, 0, "xs", dev), wp, ldw, _dense(ws, N, 0, "ws", dev), _dense(bias, N, 0, "bias", dev), T, N, K,
+                                   y.data_ptr(), sr, sn)
+    if rc:
+        check(rc, ctx.h)
     return y
 
 

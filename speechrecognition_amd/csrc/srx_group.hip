@@ -8,8 +8,6 @@
 // the output unit (dW).  Groups are ragged and known on the device only: row tile number t of the launch belongs to the group e
 // with row_off[e] / TJ + e <= t < row_off[e+1] / TJ + e + 1, a closed form that needs no table (the range holds at least the
 // ceil(rows / TJ) tiles that group e needs; the spare ones leave at once).
-#include <type_traits>
-
 #include "srx_tile.h"
 
 struct GroupArgs {
@@ -22,8 +20,7 @@ struct GroupArgs {
     int64_t total;
     int E, K, N;
     int64_t tiles_i, tiles_j;   // of the launch
-    float *part;                // dW split over rows: [S][E][N][K] then [S][E][N], f32
-    int splits;
+    float *part;                // dW's parts: two slots of TI * TJ + TJ floats per workgroup
 };
 
 __device__ __forceinline__ int64_t group_clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
@@ -51,48 +48,41 @@ __device__ __forceinline__ bool group_rows(const GroupArgs &p, int64_t t, int &e
     return true;
 }
 
+__device__ __forceinline__ void pass_four(const float (&v)[4], Nothing, f32x4_t &r) { r = {v[0], v[1], v[2], v[3]}; }
+
 // forward (DX false): i = output unit, reduction over K; dx: i = input unit, reduction over N, W read along its columns
 template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, bool DMA>
-__global__ __launch_bounds__(WI *WJ * 64) void k_group(GroupArgs p) {
+__global__ __launch_bounds__(WI *WJ * 64, 2) void k_group(GroupArgs p) {
     typedef Tile<El, WI, WJ, FI, FJ, DX, false, DMA> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
-    int64_t ti, tj;
+    struct Held {
+        float i[RUN<O>];   // bias
+        Nothing j[FJ];
+    };
+    const int I = DX ? p.K : p.N;
+    int64_t ti, tj, r0;
     tile_of(blockIdx.x, p.tiles_i, p.tiles_j, ti, tj);
-    const int i0 = (int)ti * T::TI;
     int e, rows;
-    int64_t r0;
     if (!group_rows<T::TJ>(p, tj, e, r0, rows)) return;
-    const int I = DX ? p.K : p.N, R = DX ? p.N : p.K;
+    const int i0 = (int)ti * T::TI, ni = I - i0 < T::TI ? I - i0 : T::TI;
+    Held held;
+    const int i = T::template lane_i<O>();
+#pragma unroll
+    for (int q = 0; q < RUN<O>; q++) held.i[q] = !DX && p.bias && i + q < ni ? p.bias[(int64_t)e * p.N + i0 + i + q] : 0.0f;
     const El *w = reinterpret_cast<const El *>(p.w) + (int64_t)e * p.N * p.K;
     const int64_t ldq = DX ? p.ld_dy : p.ld_x;
-    TileOperand P, Q;
-    P.base = DX ? w + i0 : w + (int64_t)i0 * p.K;
-    P.ld = p.K;
-    P.n = I - i0 < T::TI ? I - i0 : T::TI;
-    Q.base = reinterpret_cast<const El *>(DX ? p.dy : p.x) + r0 * ldq;
-    Q.ld = ldq;
-    Q.n = rows;
+    const TileOperand P{DX ? w + i0 : w + (int64_t)i0 * p.K, p.K, ni};
+    const TileOperand Q{reinterpret_cast<const El *>(DX ? p.dy : p.x) + r0 * ldq, ldq, rows};
     typename T::acc_t acc[FI][FJ];
     float none[FJ];
-    T::template product<false>(smem, P, Q, R, acc, none, false);
-    O *y = reinterpret_cast<O *>(p.y);
-    const float *bias = !DX && p.bias ? p.bias + (int64_t)e * p.N : nullptr;
-    struct Held { float b[RUN<O>]; };
-    T::template write_out<RUN<O>>(
-        smem, acc,
-        [&](int i) {
-            Held h;
+    T::template product<false>(smem, P, Q, DX ? p.N : p.K, acc, none, false);
+    T::template write_out<O>(
+        smem, acc, held, pass_four,
+        [](const float (&v)[RUN<O>], const float (&bias)[RUN<O>], auto &&, float (&r)[RUN<O>]) {
 #pragma unroll
-            for (int q = 0; q < RUN<O>; q++) h.b[q] = bias && i0 + i + q < I ? bias[i0 + i + q] : 0.0f;
-            return h;
+            for (int q = 0; q < RUN<O>; q++) r[q] = v[q] + bias[q];
         },
-        [&](int i, int j, const float (&v)[RUN<O>], const Held &h) {
-            if (j >= rows || i0 + i >= I) return;
-            float f[RUN<O>];
-#pragma unroll
-            for (int q = 0; q < RUN<O>; q++) f[q] = v[q] + h.b[q];
-            store_run<O>(y + (r0 + j) * p.ld_y + i0 + i, f, I - i0 - i);
-        });
+        TileOut<O, T::TI>(reinterpret_cast<O *>(p.y) + r0 * p.ld_y + i0, p.ld_y, ni, rows, ni == T::TI && rows == T::TJ));
 }
 
 // forward, few rows per group: tiles of 32 x 32
@@ -117,70 +107,168 @@ __global__ __launch_bounds__(THIN_WAVES * 64) void k_group_thin(GroupArgs p) {
     });
 }
 
-// dW (i = input unit k, j = output unit n, reduction over the group's rows) and db with it, taken by the tiles of i = 0 from the
-// fragments that they hold anyway.  blockIdx.y: the group; blockIdx.z: the part of its rows.
-template <class El, class O, int WI, int WJ, int FI, int FJ, bool DMA>
-__global__ __launch_bounds__(WI *WJ * 64) void k_group_dw(GroupArgs p) {
-    typedef Tile<El, WI, WJ, FI, FJ, true, true, DMA> T;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
-    int64_t ti, tj;
-    tile_of(blockIdx.x, p.tiles_i, p.tiles_j, ti, tj);
-    const int i0 = (int)ti * T::TI, j0 = (int)tj * T::TJ;
-    const int e = blockIdx.y, z = blockIdx.z;
+// dW (i = input unit k, j = output unit n, reduction over the group's rows), and db with it, taken by the tiles of i = 0 from the
+// fragments that they hold anyway.
+//
+// Groups differ in rows, so tiles differ in work: the workgroups share the slabs instead.  In the order (group, tile, slab) every
+// workgroup takes a run of equal length; a tile that one workgroup has to itself goes to its place, the two that its run may cut
+// leave their part in f32 in its scratch (slot 0: begun by another, slot 1: left to another), and k_group_join adds the parts in
+// their order.  A group of no rows counts as one slab, so that its tiles are written (zeros).
+template <int KS>
+__device__ __forceinline__ int64_t dw_slabs(const GroupArgs &p, int e) {
     const int64_t a = group_clamp(p.off[e], 0, p.total), b = group_clamp(p.off[e + 1], a, p.total);
-    const int64_t per = ((b - a + p.splits - 1) / p.splits + T::KS - 1) / T::KS * T::KS;
-    const int64_t lo = a + z * per < b ? a + z * per : b, hi = lo + per < b ? lo + per : b;
-    TileOperand P, Q;
-    P.base = reinterpret_cast<const El *>(p.x) + lo * p.ld_x + i0;
-    P.ld = p.ld_x;
-    P.n = p.K - i0 < T::TI ? p.K - i0 : T::TI;
-    Q.base = reinterpret_cast<const El *>(p.dy) + lo * p.ld_dy + j0;
-    Q.ld = p.ld_dy;
-    Q.n = p.N - j0 < T::TJ ? p.N - j0 : T::TJ;
-    typename T::acc_t acc[FI][FJ];
-    float sums[FJ];
-    const bool want = p.dbias != nullptr && i0 == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WI == 0;
-    T::template product<true>(smem, P, Q, hi - lo, acc, sums, want);
-    const bool split = p.splits > 1;
-    if (want) {
-        const int lane = threadIdx.x & 63, wj = (threadIdx.x >> 6) / WI;
-        float *db = split ? p.part + (int64_t)p.splits * p.E * p.N * p.K + ((int64_t)z * p.E + e) * p.N : p.dbias + (int64_t)e * p.N;
-#pragma unroll
-        for (int f = 0; f < FJ; f++) {
-            const float s = sums[f] + __shfl_xor(sums[f], 32);
-            const int j = j0 + (wj * FJ + f) * 32 + (lane & 31);
-            if (lane < 32 && j < p.N) db[j] = s;
-        }
-    }
-    const auto out = [&](auto *o) {
-        typedef std::remove_reference_t<decltype(*o)> Out;
-        T::template write_out<RUN<Out>>(
-            smem, acc, [](int) { return 0; },
-            [&](int i, int j, const float (&v)[RUN<Out>], int) {
-                if (j0 + j < p.N && i0 + i < p.K) store_run<Out>(o + (int64_t)(j0 + j) * p.K + i0 + i, v, p.K - i0 - i);
-            });
-    };
-    if (split) out(p.part + ((int64_t)z * p.E + e) * p.N * p.K);
-    else out(reinterpret_cast<O *>(p.y) + (int64_t)e * p.N * p.K);
+    return b > a ? (b - a + KS - 1) / KS : 1;
 }
 
-// The parts of dW and db, added in their order
-template <class O>
-__global__ __launch_bounds__(256) void k_group_join(GroupArgs p) {
-    const int64_t nw = (int64_t)p.E * p.N * p.K, nb = p.dbias ? (int64_t)p.E * p.N : 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nw + nb; i += (int64_t)gridDim.x * 256) {
-        const float *q = i < nw ? p.part + i : p.part + (int64_t)p.splits * nw + (i - nw);
-        const int64_t step = i < nw ? nw : (int64_t)p.E * p.N;
-        float s = 0.0f;
-        for (int z = 0; z < p.splits; z++) s += q[z * step];
-        if (i < nw) reinterpret_cast<O *>(p.y)[i] = srx_from_f32<O>(s);
-        else p.dbias[i - nw] = s;
+// The same number in every lane, known to the compiler as such: operand addresses are scalar
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// total: slabs of all groups' tiles; len: those of each of the G runs; e: the group in which run `me` begins, and `before`: the
+// slabs of the groups before it (of one tile).  Every thread of the workgroup counts a run of groups; sh: a number per thread.
+template <int KS, int NT>
+__device__ __forceinline__ void dw_find(const GroupArgs &p, int64_t *sh, int64_t tiles, int64_t me, int64_t G, int64_t &total, int64_t &len, int &e, int64_t &before) {
+    const int t = threadIdx.x, each = (p.E + NT - 1) / NT;
+    const int g0 = t * each < p.E ? t * each : p.E, g1 = g0 + each < p.E ? g0 + each : p.E;
+    int64_t mine = 0;
+    for (int g = g0; g < g1; g++) mine += dw_slabs<KS>(p, g);
+    sh[t] = mine;
+    __syncthreads();
+    int64_t front = 0, all = 0;
+    for (int i = 0; i * each < p.E; i++) {
+        const int64_t v = sh[i];
+        if (i < t) front += v;
+        all += v;
+    }
+    __syncthreads();
+    total = uniform64(all) * tiles;
+    len = (total + G - 1) / G;
+    const int64_t at = me * len / tiles;   // in slabs of groups
+    if (g0 < g1 && front <= at && at < front + mine) {
+        int g = g0;
+        int64_t f = front;
+        for (; g + 1 < g1; g++) {
+            const int64_t n = dw_slabs<KS>(p, g);
+            if (f + n > at) break;
+            f += n;
+        }
+        sh[0] = g;
+        sh[1] = f;
+    }
+    __syncthreads();
+    e = (int)uniform64(sh[0]);
+    before = uniform64(sh[1]);
+    __syncthreads();
+}
+
+template <class El, class O, int WI, int WJ, int FI, int FJ, bool DMA>
+__global__ __launch_bounds__(WI *WJ * 64, 2) void k_group_dw(GroupArgs p) {
+    typedef Tile<El, WI, WJ, FI, FJ, true, true, DMA> T;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
+    constexpr int64_t SLOT = T::TI * T::TJ + T::TJ;   // (whole lines: a multiple of 128 bytes)
+    struct Held { Nothing i[1], j[FJ]; };
+    const int64_t tiles = p.tiles_i * p.tiles_j;
+    // workgroups of one XCD take neighbouring runs: the tiles of the same rows share its L2
+    const int64_t G = gridDim.x, x = blockIdx.x % 8, q8 = G / 8, r8 = G % 8;
+    const int64_t me = x * q8 + (x < r8 ? x : r8) + blockIdx.x / 8;
+    int64_t total, len, before;
+    int e;
+    dw_find<T::KS, T::NT>(p, reinterpret_cast<int64_t *>(smem), tiles, me, G, total, len, e, before);
+    int64_t at = me * len;
+    const int64_t end = at + len < total ? at + len : total;
+    while (at < end) {
+        int64_t n = dw_slabs<T::KS>(p, e);
+        while (at >= (before + n) * tiles) {
+            before += n;
+            e++;
+            n = dw_slabs<T::KS>(p, e);
+        }
+        const int64_t in = at - before * tiles, tile = in / n, s0 = in - tile * n;
+        const int64_t s1 = s0 + (end - at) < n ? s0 + (end - at) : n;
+        const int64_t a = group_clamp(p.off[e], 0, p.total), b = group_clamp(p.off[e + 1], a, p.total);
+        const int64_t lo = a + s0 * T::KS < b ? a + s0 * T::KS : b, hi = a + s1 * T::KS < b ? a + s1 * T::KS : b;
+        const int64_t tj = tile / p.tiles_i;
+        const int i0 = (int)(tile - tj * p.tiles_i) * T::TI, j0 = (int)tj * T::TJ;
+        const TileOperand P{reinterpret_cast<const El *>(p.x) + lo * p.ld_x + i0, p.ld_x, p.K - i0 < T::TI ? p.K - i0 : T::TI};
+        const TileOperand Q{reinterpret_cast<const El *>(p.dy) + lo * p.ld_dy + j0, p.ld_dy, p.N - j0 < T::TJ ? p.N - j0 : T::TJ};
+        const int slot = s0 > 0 ? 0 : s1 < n ? 1 : -1;   // -1: the whole reduction
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const bool wants = p.dbias != nullptr && i0 == 0 && wave % WI == 0;
+        typename T::acc_t acc[FI][FJ];
+        float sums[FJ];
+        T::template product<true>(smem, P, Q, hi - lo, acc, sums, wants);
+        float *part = p.part + (me * 2 + (slot > 0)) * SLOT;
+        if (wants) {
+            const int lane = threadIdx.x & 63;
+#pragma unroll
+            for (int f = 0; f < FJ; f++) {
+                const float v = sums[f] + __shfl_xor(sums[f], 32);
+                const int j = (wave / WI * FJ + f) * 32 + (lane & 31);
+                if (lane < 32) {
+                    if (slot >= 0) part[T::TI * T::TJ + j] = v;
+                    else if (j0 + j < p.N) p.dbias[(int64_t)e * p.N + j0 + j] = v;
+                }
+            }
+        }
+        const auto same = [](const auto &v, const Nothing (&)[1], auto &&, auto &r) {
+#pragma unroll
+            for (int q = 0; q < (int)(sizeof(v) / sizeof(v[0])); q++) r[q] = v[q];
+        };
+        if (slot >= 0) T::template write_out<float>(smem, acc, Held{}, pass_four, same, TileOut<float, T::TI, false>(part, T::TI, T::TI, T::TJ, true));
+        else
+            T::template write_out<O>(smem, acc, Held{}, pass_four, same,
+                                     TileOut<O, T::TI>(reinterpret_cast<O *>(p.y) + ((int64_t)e * p.N + j0) * p.K + i0, p.K, P.n, Q.n, P.n == T::TI && Q.n == T::TJ));
+        at += s1 - s0;
+        lds_barrier();   // (the next product's loads go where columns were taken from)
+    }
+}
+
+// Workgroup g of k_group_dw's G begins inside a tile: if it is the first to do so, this one adds the tile's parts -- slot 1 of the
+// workgroup before it, slot 0 of itself and of those that follow up to the tile's end.  blockIdx.y: JOIN_COLS of the tile's columns.
+static constexpr int JOIN_COLS = 8;
+
+template <class O, int TI, int TJ, int KS>
+__global__ __launch_bounds__(256) void k_group_join(GroupArgs p, int64_t G) {
+    __shared__ int64_t sh[256];
+    constexpr int64_t SLOT = TI * TJ + TJ;
+    const int64_t tiles = p.tiles_i * p.tiles_j, g = blockIdx.x + 1;
+    int64_t total, len, before;
+    int e;
+    dw_find<KS, 256>(p, sh, tiles, g, G, total, len, e, before);
+    const int64_t at = g * len;
+    if (at >= total) return;
+    const int64_t n = dw_slabs<KS>(p, e), tile = (at - before * tiles) / n, first = before * tiles + tile * n;
+    if (at == first || at - len > first) return;   // begins with the tile, or is not the first inside it
+    const int64_t parts = (first + n - 1) / len - g + 2;   // g - 1, g, .. the one that holds the tile's last slab
+    const int64_t tj = tile / p.tiles_i;
+    const int i0 = (int)(tile - tj * p.tiles_i) * TI, j0 = (int)tj * TJ;
+    const float *slot = p.part + ((g - 1) * 2 + 1) * SLOT;
+    constexpr int ROWS = JOIN_COLS;
+    for (int c = threadIdx.x; c < ROWS * (TI / 4); c += 256) {
+        const int j = blockIdx.y * ROWS + c / (TI / 4), i = c % (TI / 4) * 4;
+        if (j0 + j >= p.N || i0 + i >= p.K) continue;
+        f32x4_t v = *reinterpret_cast<const f32x4_t *>(slot + j * TI + i);
+#pragma unroll 4
+        for (int64_t q = 1; q < parts; q++) v += *reinterpret_cast<const f32x4_t *>(slot + (2 * q - 1) * SLOT + j * TI + i);
+        const float f[4] = {v[0], v[1], v[2], v[3]};
+        store_four<O>(reinterpret_cast<O *>(p.y) + ((int64_t)e * p.N + j0 + j) * p.K + i0 + i, f, p.K - i0 - i);
+    }
+    if (p.dbias && i0 == 0 && (int)threadIdx.x < ROWS) {
+        const int j = blockIdx.y * ROWS + threadIdx.x;
+        if (j0 + j < p.N) {
+            float v = slot[TI * TJ + j];
+            for (int64_t q = 1; q < parts; q++) v += slot[(2 * q - 1) * SLOT + TI * TJ + j];
+            p.dbias[(int64_t)e * p.N + j0 + j] = v;
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
 static constexpr int64_t GROUP_MAX_ROWS = 1ll << 40;
 static constexpr int GROUP_MAX_DIM = 1 << 20;
+static constexpr int64_t GROUP_MAX_LD = 1 << 21;   // (a tile's 128 rows of f32 stay inside 32 bits)
 
 static int group_check(srx_ctx *ctx, const char *name, int in_dtype, int out_dtype, int E, int64_t total, int K, int N) {
     SRX_REQUIRE(ctx, srx_dtype_size(in_dtype) != 0 && (out_dtype == in_dtype || out_dtype == SRX_F32), "%s: element types %d -> %d (out: the same or f32)", name,
@@ -199,7 +287,7 @@ static int group_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
     typedef Tile<El, WI, WJ, FI, FJ, DX, false, DMA> T;
     p.tiles_i = ceil_div64(DX ? p.K : p.N, T::TI);
     p.tiles_j = p.total / T::TJ + p.E;
-    SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31), "%s: too many tiles", name);
+    SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
     SrxProf prof_(ctx, DX ? "k_group_dx" : "k_group");
     hipLaunchKernelGGL((k_group<El, O, DX, WI, WJ, FI, FJ, DMA>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
     return SRX_OK;
@@ -213,7 +301,7 @@ static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
         if (p.total <= THIN_ROWS * p.E) {
             p.tiles_i = ceil_div64(p.N, 32);
             p.tiles_j = p.total / 32 + p.E;
-            SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31), "%s: too many tiles", name);
+            SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
             SrxProf prof_(ctx, "k_group_thin");
             hipLaunchKernelGGL((k_group_thin<El, O>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(THIN_WAVES * 64), 0, ctx->stream, p);
             return SRX_OK;
@@ -245,7 +333,7 @@ extern "C" int srx_group_matmul_dev(srx_ctx *ctx, int in_dtype, int out_dtype, c
     int rc = group_check(ctx, name, in_dtype, out_dtype, n_groups, total_rows, K, N);
     if (rc != SRX_OK || n_groups == 0 || total_rows == 0) return rc;
     SRX_REQUIRE(ctx, x_dev && w_dev && row_off_dev && y_dev, "%s: null argument", name);
-    SRX_REQUIRE(ctx, ld_x >= K && ld_y >= N, "%s: a row stride below its %d / %d columns", name, K, N);
+    SRX_REQUIRE(ctx, ld_x >= K && ld_y >= N && ld_x <= GROUP_MAX_LD && ld_y <= GROUP_MAX_LD, "%s: row strides %lld, %lld for %d / %d columns", name, (long long)ld_x, (long long)ld_y, K, N);
     SRX_REQUIRE(ctx, srx_aligned(x_dev, srx_dtype_size(in_dtype)) && srx_aligned(w_dev, srx_dtype_size(in_dtype)) && srx_aligned(y_dev, srx_dtype_size(out_dtype)),
                 "%s: misaligned buffer", name);
     GroupArgs p{};
@@ -261,7 +349,7 @@ extern "C" int srx_group_matmul_dx_dev(srx_ctx *ctx, int in_dtype, int out_dtype
     int rc = group_check(ctx, name, in_dtype, out_dtype, n_groups, total_rows, K, N);
     if (rc != SRX_OK || n_groups == 0 || total_rows == 0) return rc;
     SRX_REQUIRE(ctx, dy_dev && w_dev && row_off_dev && dx_dev, "%s: null argument", name);
-    SRX_REQUIRE(ctx, ld_dy >= N && ld_dx >= K, "%s: a row stride below its %d / %d columns", name, N, K);
+    SRX_REQUIRE(ctx, ld_dy >= N && ld_dx >= K && ld_dy <= GROUP_MAX_LD && ld_dx <= GROUP_MAX_LD, "%s: row strides %lld, %lld for %d / %d columns", name, (long long)ld_dy, (long long)ld_dx, N, K);
     SRX_REQUIRE(ctx, srx_aligned(dy_dev, srx_dtype_size(in_dtype)) && srx_aligned(w_dev, srx_dtype_size(in_dtype)) && srx_aligned(dx_dev, srx_dtype_size(out_dtype)),
                 "%s: misaligned buffer", name);
     GroupArgs p{};
@@ -270,35 +358,26 @@ extern "C" int srx_group_matmul_dx_dev(srx_ctx *ctx, int in_dtype, int out_dtype
     return group_types<true>(ctx, name, in_dtype, out_dtype, p);
 }
 
-// Tiles of dW, and the parts that the rows of a group are cut into where there are fewer tiles than fill the chip: the cheapest by
-// rounds of tiles (see tile_large), at least DW_MIN_ROWS rows of an average group to a part.  The sum of the parts costs about
-// DW_JOIN of a round of an average group's rows for each part's E N K.
-struct DwPlan { bool large; int splits; };
-static constexpr int64_t DW_MIN_ROWS = 512, DW_CUS = 256;
+// dW: workgroups (as many as the chip holds at a time, fewer where a share would be below DW_SLABS slabs) and the size of a part
+static constexpr int64_t DW_SLABS = 4;
 
-static DwPlan group_dw_plan(int E, int64_t total, int K, int N) {
-    const int64_t nl = E * ceil_div64(K, 256) * ceil_div64(N, 256), ns = E * ceil_div64(K, 128) * ceil_div64(N, 128);
-    int64_t most = total / E / DW_MIN_ROWS;
-    most = most < 1 ? 1 : most > 64 ? 64 : most;
-    DwPlan best{false, 1};
-    double cost = 1e300;
-    // a round of whole groups of R rows, large tiles: about R * 28 ns (8,192 rows: 230 us); a part's write and read again at
-    // 4 TB/s
-    const double R = (double)total / E * 28e-9, part = 8.0 * E * N * (double)K / 4e12;
-    for (int64_t s = 1; s <= most; s++) {
-        const double join = s > 1 ? s * part + 4e-6 : 0.0;
-        const double l = (double)ceil_div64(nl * s, DW_CUS) * R / s + join, m = 0.63 * (double)ceil_div64(ns * s, 2 * DW_CUS) * R / s + join;
-        if (l < cost) { cost = l; best = {true, (int)s}; }
-        if (m < cost) { cost = m; best = {false, (int)s}; }
-    }
-    return best;
+static int64_t dw_groups(const srx_ctx *ctx, int E, int64_t total, int K, int N, int tile, int ks) {
+    const int64_t slabs = (total / ks + E) * ceil_div64(K, tile) * ceil_div64(N, tile), most = (int64_t)ctx->num_cus * (tile == 256 ? 1 : 2);
+    const int64_t g = ceil_div64(slabs, DW_SLABS);
+    return g < 1 ? 1 : g < most ? g : most;
+}
+static int64_t dw_bytes(int64_t groups, int tile) { return groups < 2 ? 0 : groups * 2 * (tile * tile + tile) * (int64_t)sizeof(float); }
+// 256 x 256 tiles where they cover no more than 128 x 128 ones do, and there is work for more than a slab or two each
+static bool dw_large(const srx_ctx *ctx, int E, int64_t total, int K, int N) {
+    return ceil_div64(K, 256) * ceil_div64(N, 256) * 4 * 4 <= ceil_div64(K, 128) * ceil_div64(N, 128) * 5 &&
+           (total / 64 + E) * ceil_div64(K, 256) * ceil_div64(N, 256) >= 8 * (int64_t)ctx->num_cus;
 }
 
 extern "C" int64_t srx_group_matmul_dw_scratch_bytes(const srx_ctx *ctx, int n_groups, int64_t total_rows, int K, int N) {
     if (!ctx || n_groups < 0 || n_groups > (1 << 20) || total_rows < 0 || total_rows > GROUP_MAX_ROWS || K < 1 || N < 1 || K > GROUP_MAX_DIM || N > GROUP_MAX_DIM) return -1;
     if (n_groups == 0) return 0;
-    const int64_t s = group_dw_plan(n_groups, total_rows, K, N).splits;
-    return s == 1 ? 0 : s * n_groups * N * ((int64_t)K + 1) * (int64_t)sizeof(float);
+    const int64_t large = dw_bytes(dw_groups(ctx, n_groups, total_rows, K, N, 256, 32), 256), small = dw_bytes(dw_groups(ctx, n_groups, total_rows, K, N, 128, 32), 128);
+    return dw_large(ctx, n_groups, total_rows, K, N) && large > small ? large : small;   // (the larger slab counts of f32 bound the other types')
 }
 
 template <class El, class O, int WI, int WJ, int FI, int FJ, bool DMA>
@@ -306,23 +385,22 @@ static int group_dw_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
     typedef Tile<El, WI, WJ, FI, FJ, true, true, DMA> T;
     p.tiles_i = ceil_div64(p.K, T::TI);
     p.tiles_j = ceil_div64(p.N, T::TJ);
-    SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31) && p.E <= 65535, "%s: too many tiles", name);
-    SrxProf prof_(ctx, "k_group_dw");
-    hipLaunchKernelGGL((k_group_dw<El, O, WI, WJ, FI, FJ, DMA>), dim3((unsigned)(p.tiles_i * p.tiles_j), (unsigned)p.E, (unsigned)p.splits), dim3(T::NT), 0, ctx->stream, p);
+    const int64_t G = dw_groups(ctx, p.E, p.total, p.K, p.N, T::TI, T::KS);
+    {
+        SrxProf prof_(ctx, "k_group_dw");
+        hipLaunchKernelGGL((k_group_dw<El, O, WI, WJ, FI, FJ, DMA>), dim3((unsigned)G), dim3(T::NT), 0, ctx->stream, p);
+    }
+    if (G > 1) {
+        SrxProf prof_(ctx, "k_group_join");
+        hipLaunchKernelGGL((k_group_join<O, T::TI, T::TJ, T::KS>), dim3((unsigned)(G - 1), T::TJ / JOIN_COLS), dim3(256), 0, ctx->stream, p, G);
+    }
     return SRX_OK;
 }
 
 template <class El, class O>
-static int group_dw_launch(srx_ctx *ctx, const char *name, GroupArgs &p, bool large) {
-    const bool dma = tile_dma(p.x, p.ld_x, p.K, sizeof(El)) && tile_dma(p.dy, p.ld_dy, p.N, sizeof(El));
-    const int rc = !dma ? group_dw_tile<El, O, 2, 2, 2, 2, false>(ctx, name, p)
-                 : large ? group_dw_tile<El, O, 2, 4, 4, 2, true>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, true>(ctx, name, p);
-    if (rc == SRX_OK && p.splits > 1) {
-        const int64_t n = ceil_div64((int64_t)p.E * p.N * (p.K + 1ll), 256);
-        SrxProf prof_(ctx, "k_group_join");
-        hipLaunchKernelGGL((k_group_join<O>), dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, ctx->stream, p);
-    }
-    return rc;
+static int group_dw_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
+    if (!tile_dma(p.x, p.ld_x, p.K, sizeof(El)) || !tile_dma(p.dy, p.ld_dy, p.N, sizeof(El))) return group_dw_tile<El, O, 2, 2, 2, 2, false>(ctx, name, p);
+    return dw_large(ctx, p.E, p.total, p.K, p.N) ? group_dw_tile<El, O, 2, 4, 4, 2, true>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, true>(ctx, name, p);
 }
 
 extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *x_dev, int64_t ld_x,
@@ -333,23 +411,21 @@ extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype
     int rc = group_check(ctx, name, in_dtype, out_dtype, n_groups, total_rows, K, N);
     if (rc != SRX_OK || n_groups == 0) return rc;
     SRX_REQUIRE(ctx, row_off_dev && dw_dev && (total_rows == 0 || (dy_dev && x_dev)), "%s: null argument", name);
-    SRX_REQUIRE(ctx, ld_dy >= N && ld_x >= K, "%s: a row stride below its %d / %d columns", name, N, K);
+    SRX_REQUIRE(ctx, ld_dy >= N && ld_x >= K && ld_dy <= GROUP_MAX_LD && ld_x <= GROUP_MAX_LD, "%s: row strides %lld, %lld for %d / %d columns", name, (long long)ld_dy, (long long)ld_x, N, K);
     SRX_REQUIRE(ctx, srx_aligned(dy_dev, srx_dtype_size(in_dtype)) && srx_aligned(x_dev, srx_dtype_size(in_dtype)) && srx_aligned(dw_dev, srx_dtype_size(out_dtype)),
                 "%s: misaligned buffer", name);
     GroupArgs p{};
     p.dy = dy_dev; p.ld_dy = ld_dy; p.x = x_dev; p.ld_x = ld_x; p.y = dw_dev; p.dbias = dbias_dev;
     p.off = row_off_dev; p.total = total_rows; p.E = n_groups; p.K = K; p.N = N;
-    const DwPlan plan = group_dw_plan(n_groups, total_rows, K, N);
-    p.splits = plan.splits;
     const int64_t need = srx_group_matmul_dw_scratch_bytes(ctx, n_groups, total_rows, K, N);
     if (need) {
         SRX_REQUIRE(ctx, scratch_dev && scratch_bytes >= need && srx_aligned(scratch_dev, 16), "%s: scratch of %lld bytes, %lld needed, 16-byte aligned (srx_group_matmul_dw_scratch_bytes)",
                     name, (long long)(scratch_dev ? scratch_bytes : 0), (long long)need);
         p.part = reinterpret_cast<float *>(scratch_dev);
     }
-    if (in_dtype == SRX_F32) rc = group_dw_launch<float, float>(ctx, name, p, plan.large);
-    else if (in_dtype == SRX_F16) rc = out_dtype == SRX_F32 ? group_dw_launch<srx_f16, float>(ctx, name, p, plan.large) : group_dw_launch<srx_f16, srx_f16>(ctx, name, p, plan.large);
-    else rc = out_dtype == SRX_F32 ? group_dw_launch<srx_bf16, float>(ctx, name, p, plan.large) : group_dw_launch<srx_bf16, srx_bf16>(ctx, name, p, plan.large);
+    if (in_dtype == SRX_F32) rc = group_dw_launch<float, float>(ctx, name, p);
+    else if (in_dtype == SRX_F16) rc = out_dtype == SRX_F32 ? group_dw_launch<srx_f16, float>(ctx, name, p) : group_dw_launch<srx_f16, srx_f16>(ctx, name, p);
+    else rc = out_dtype == SRX_F32 ? group_dw_launch<srx_bf16, float>(ctx, name, p) : group_dw_launch<srx_bf16, srx_bf16>(ctx, name, p);
     if (rc != SRX_OK) return rc;
     SRX_LAUNCH_CHECK(ctx);
     return SRX_OK;

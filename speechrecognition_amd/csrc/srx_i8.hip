@@ -4,8 +4,6 @@
 //   y_rn = s_r s_n sum_k q_rk q_nk + b_n
 //
 // The sum is exact in 32 bits (K <= SRX_I8_MAX_K), so the only roundings are the scale's, the codes' and the output's few.
-#include <type_traits>
-
 #include "srx_tile.h"
 
 struct QuantArgs {
@@ -139,40 +137,44 @@ struct I8Args {
     int64_t tiles_i, tiles_j;
 };
 
+struct ScaleBias { float s, b; };
+__device__ __forceinline__ ScaleBias from_lane(const ScaleBias &v, int l) { return {__shfl(v.s, l), __shfl(v.b, l)}; }
+
 template <class O, int WI, int WJ, int FI, int FJ>
-__global__ __launch_bounds__(WI *WJ * 64) void k_matmul_i8(I8Args p) {
+__global__ __launch_bounds__(WI *WJ * 64, 2) void k_matmul_i8(I8Args p) {
     typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, true> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
+    struct Held { ScaleBias i[RUN<O>], j[FJ]; };
     int64_t i0, j0;
     tile_of(blockIdx.x, p.tiles_i, p.tiles_j, i0, j0);
     i0 *= T::TI;
     j0 *= T::TJ;
-    TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < T::TI ? p.I - i0 : T::TI)};
-    TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < T::TJ ? p.J - j0 : T::TJ)};
+    const TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < T::TI ? p.I - i0 : T::TI)};
+    const TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < T::TJ ? p.J - j0 : T::TJ)};
+    Held held;
+    const int i = T::template lane_i<O>();
+#pragma unroll
+    for (int e = 0; e < RUN<O>; e++) held.i[e] = {i + e < P.n ? p.sp[i0 + i + e] : 0.0f, p.bias && p.bias_i && i + e < P.n ? p.bias[i0 + i + e] : 0.0f};
+#pragma unroll
+    for (int c = 0; c < FJ; c++) {
+        const int j = T::lane_j(c);
+        held.j[c] = {j < Q.n ? p.sq[j0 + j] : 0.0f, p.bias && !p.bias_i && j < Q.n ? p.bias[j0 + j] : 0.0f};
+    }
     typename T::acc_t acc[FI][FJ];
     float none[FJ];
     T::template product<false>(smem, P, Q, (p.K + 15) / 16 * 16, acc, none, false);
-    O *y = reinterpret_cast<O *>(p.y);
-    struct Held { float s[RUN<O>], b[RUN<O>]; };
-    T::template write_out<RUN<O>>(
-        smem, acc,
-        [&](int i) {
-            Held h;
+    T::template write_out<O>(
+        smem, acc, held, [](const float (&v)[4], const ScaleBias &j, f32x4_t &r) { r = {v[0] * j.s, v[1] * j.s, v[2] * j.s, v[3] * j.s}; },
+        [&](const float (&v)[RUN<O>], const ScaleBias (&i)[RUN<O>], auto &&j, float (&r)[RUN<O>]) {
 #pragma unroll
-            for (int e = 0; e < RUN<O>; e++) {
-                h.s[e] = i + e < P.n ? p.sp[i0 + i + e] : 0.0f;
-                h.b[e] = p.bias && p.bias_i && i + e < P.n ? p.bias[i0 + i + e] : 0.0f;
+            for (int e = 0; e < RUN<O>; e++) r[e] = __builtin_fmaf(v[e], i[e].s, i[e].b);
+            if (!p.bias_i) {
+                const float b = j().b;
+#pragma unroll
+                for (int e = 0; e < RUN<O>; e++) r[e] += b;
             }
-            return h;
         },
-        [&](int i, int j, const float (&v)[RUN<O>], const Held &h) {
-            if (j >= Q.n || i >= P.n) return;
-            const float sj = p.sq[j0 + j], bj = p.bias && !p.bias_i ? p.bias[j0 + j] : 0.0f;
-            float f[RUN<O>];
-#pragma unroll
-            for (int e = 0; e < RUN<O>; e++) f[e] = __builtin_fmaf(v[e] * sj, h.s[e], p.bias_i ? h.b[e] : bj);
-            store_run<O>(y + (j0 + j) * p.ld_y + i0 + i, f, P.n - i);
-        });
+        TileOut<O, T::TI>(reinterpret_cast<O *>(p.y) + j0 * p.ld_y + i0, p.ld_y, P.n, Q.n, P.n == T::TI && Q.n == T::TJ));
 }
 
 // Few rows: tiles of 32 x 32
@@ -246,7 +248,7 @@ static int i8_tile(srx_ctx *ctx, const char *name, I8Args &p) {
     typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, true> T;
     p.tiles_i = ceil_div64(p.I, T::TI);
     p.tiles_j = ceil_div64(p.J, T::TJ);
-    SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 31), "%s: too many tiles", name);
+    SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
     SrxProf prof_(ctx, "k_matmul_i8");
     hipLaunchKernelGGL((k_matmul_i8<O, WI, WJ, FI, FJ>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
     return SRX_OK;
@@ -278,7 +280,7 @@ extern "C" int srx_matmul_i8_dev(srx_ctx *ctx, int out_dtype, const int8_t *xq_d
     const int k16 = (K + 15) / 16 * 16;
     SRX_REQUIRE(ctx, ld_xq >= k16 && ld_wq >= k16 && ld_xq % 16 == 0 && ld_wq % 16 == 0 && ld_xq <= (1 << 22) && ld_wq <= (1 << 22) && srx_aligned(xq_dev, 16) && srx_aligned(wq_dev, 16),
                 "%s: code rows of %lld / %lld bytes for K = %d (whole 16 bytes, 16-byte aligned, at most 4 MiB)", name, (long long)ld_xq, (long long)ld_wq, K);
-    SRX_REQUIRE(ctx, (stride_n == 1 && stride_r >= N) || (stride_r == 1 && stride_n >= rows), "%s: output strides %lld, %lld (one of them 1)", name, (long long)stride_r,
+    SRX_REQUIRE(ctx, (stride_n == 1 && stride_r >= N && stride_r <= (1 << 26)) || (stride_r == 1 && stride_n >= rows && stride_n <= (1 << 26)), "%s: output strides %lld, %lld (one of them 1, the other at most 2^26 and no less than what it crosses)", name, (long long)stride_r,
                 (long long)stride_n);
     SRX_REQUIRE(ctx, srx_aligned(y_dev, srx_dtype_size(out_dtype)), "%s: misaligned buffer", name);
     I8Args p{};

@@ -17,6 +17,8 @@
 //
 // Result layout: lane l holds column j = l & 31, rows 8 b + 4 (l >> 5) + 0..3 for b = 0..3: four adjacent i for one j.
 #pragma once
+#include <type_traits>
+
 #include "srx_dtype.h"
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -81,7 +83,7 @@ struct TileLoader {
     int64_t ldb;         // bytes per row of memory
     int n;
     int64_t K;
-    unsigned off[PER];   // chunk's byte offset from the slab's first row / column
+    unsigned off[PER];   // the chunk's byte offset from the slab's first row / column
     int kin[PER];        // rows: first k of the chunk in its slab; columns: its k
     int col[PER];        // rows: its row; columns: its first column
 
@@ -123,11 +125,12 @@ struct TileLoader {
     }
     // Any alignment and size: whole chunks by one (unaligned) 16-byte load, the rest element by element
     __device__ __forceinline__ void load(int64_t k0, i32x4_t (&v)[PER]) const {
+        const char *b = base + k0 * (COLS ? ldb : Z);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int64_t k = k0 + kin[i];
-            const int64_t have = COLS ? (k < K ? (int64_t)n - col[i] : 0) : (col[i] < n ? K - k : 0);
-            const char *p = COLS ? base + k * ldb + (int64_t)col[i] * Z : base + (int64_t)col[i] * ldb + k * Z;
+            const int64_t left = K - k0 - kin[i];
+            const int64_t have = COLS ? (left > 0 ? n - col[i] : 0) : (col[i] < n ? left : 0);
+            const char *p = b + off[i];   // (only where have > 0)
             i32x4_t r = {0, 0, 0, 0};
             if (have >= EPC) __builtin_memcpy(&r, p, 16);
             else if (have > 0) {
@@ -144,6 +147,8 @@ struct TileLoader {
         for (int i = 0; i < PER; i++) *reinterpret_cast<__attribute__((address_space(3))) i32x4_t *>(dst + (t + i * NT) * 16) = v[i];
     }
 };
+
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // A lane's fragments of one operand, `first`: the wave's first row / column in the tile
 template <class El, bool COLS, int TX>
@@ -183,7 +188,16 @@ struct TileReader {
     }
 };
 
-// WI x WJ waves of FI x FJ fragments of 32 x 32.  DMA: see TileLoader::dma for what the host has to have checked.
+// Elements per 16-byte run of an output type
+template <class O>
+static constexpr int RUN = 16 / sizeof(O);
+
+// Lane l's value
+__device__ __forceinline__ float from_lane(float v, int l) { return __shfl(v, l); }
+struct Nothing {};
+__device__ __forceinline__ Nothing from_lane(Nothing, int) { return {}; }
+
+// WI x WJ waves of FI x FJ fragments of 32 x 32.  DMA: see TileLoader::slab for what the host has to have checked.
 template <class El, int WI_, int WJ_, int FI_, int FJ_, bool PC, bool QC, bool DMA>
 struct Tile {
     static constexpr int WI = WI_, WJ = WJ_, FI = FI_, FJ = FJ_;
@@ -192,10 +206,11 @@ struct Tile {
     static constexpr int STAGE = (TI + TJ) * SLAB, LDS = 2 * STAGE;
     typedef typename MxType<El>::acc acc_t;
 
-    // SUM: also sums[f] += sum over k of Q[j][k] for the lane's column of fragment f, its half-wave's part (sum_on: wanted)
+    // acc = the tile's sums.  SUM: sums[f] = sum over k of Q[j][k] for the lane's column of fragment f, its half-wave's part, where
+    // sum_on.  LDS is free on return.
     template <bool SUM>
-    static __device__ __forceinline__ void product(unsigned char *smem, const TileOperand &P, const TileOperand &Q, int64_t K, acc_t (&acc)[FI][FJ],
-                                                   float (&sums)[FJ], bool sum_on) {
+    static __device__ __forceinline__ void product(unsigned char *smem, const TileOperand &P, const TileOperand &Q, int64_t K, acc_t (&acc)[FI][FJ], float (&sums)[FJ],
+                                                   bool sum_on) {
 #if defined(__HIP_DEVICE_COMPILE__)   // (the compiler's host pass does not know all of the builtins)
         const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
         const int wi = wave % WI, wj = wave / WI;
@@ -204,20 +219,8 @@ struct Tile {
         TileLoader<El, QC, TJ, NT> lq;
         TileReader<El, PC, TI> rp;
         TileReader<El, QC, TJ> rq;
-        lp.init(P, K, t);
-        lq.init(Q, K, t);
         rp.init(wi * FI * 32, lane);
         rq.init(wj * FJ * 32, lane);
-#pragma unroll
-        for (int i = 0; i < FI; i++)
-#pragma unroll
-            for (int j = 0; j < FJ; j++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
-#pragma unroll
-        for (int j = 0; j < FJ; j++) sums[j] = 0.0f;
-        const int64_t slabs = (K + KS - 1) / KS;
-        if (slabs <= 0) return;
         // Two slabs of LDS.  While slab s is multiplied, slab s + 1 is on its way (DMA: into the other half; otherwise: into
         // registers).  Fragments are read one k-step ahead of their products; the barrier at a slab's end stands before its last
         // k-step's products, when everything of the slab has been read, so that the next slab's first fragments and the loads of
@@ -245,10 +248,6 @@ struct Tile {
                 lq.store(vq, to + TI * SLAB, t);
             }
         };
-        ahead(0, 0);
-        settle(0);
-        tile_barrier();
-        ahead(1, 1);
         i32x4_t a[2][FI], b[2][FJ];
         auto fetch = [&](int stage, int ks, int to) __attribute__((always_inline)) {
             const lds_bytes from = lds + stage * STAGE;
@@ -276,6 +275,22 @@ struct Tile {
                     }
                 }
         };
+        lp.init(P, K, t);
+        lq.init(Q, K, t);
+        const int64_t slabs = (K + KS - 1) / KS;
+        ahead(0, 0);
+        if constexpr (DMA) ahead(1, 1);
+#pragma unroll
+        for (int i = 0; i < FI; i++)
+#pragma unroll
+            for (int j = 0; j < FJ; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
+#pragma unroll
+        for (int j = 0; j < FJ; j++) sums[j] = 0.0f;
+        settle(0);
+        tile_barrier();
+        if constexpr (!DMA) ahead(1, 1);
         fetch(0, 0, 0);
         for (int64_t s = 0; s < slabs; s++) {
             const int cur = s & 1, nxt = cur ^ 1;
@@ -316,60 +331,89 @@ struct Tile {
 #endif
     }
 
-    // Hands the tile out in runs of V adjacent i: emit(i, j, v, begin(i)) with v[0..V-1] = D[i .. i+V-1][j] in f32, i and j
-    // counted within the tile.  The accumulators' own order has four adjacent i per lane and a different j in every lane; each
-    // wave turns 32 of its columns at a time through its own part of LDS (free by now), so that the lanes of a row lie side by
-    // side: stores of whole lines (128 i of f32: 512 bytes) in place of 16-byte pieces.  A lane keeps its i for all rows.
-    template <int V, class Begin, class Emit>
-    static __device__ __forceinline__ void write_out(unsigned char *smem, const acc_t (&acc)[FI][FJ], Begin &&begin, Emit &&emit) {
-        constexpr int W = FI * 32, LPR = W / V, RPI = 64 / LPR;
-        static_assert(WI * WJ * W * 32 * 4 <= LDS && LPR <= 64, "tile shape");
+    // Writes a finished tile.  The accumulators' order has four adjacent i per lane and another j in every lane.  In passes of COLS
+    // columns per row of waves, the waves put their parts side by side into LDS (f32; chunk c of column j at c ^ (j & 7): no two
+    // lanes on one bank) and take whole columns out of it, so that a store is one run of TI outputs.  Its length matters where
+    // columns do not begin on lines of 128 bytes (2,000 f32 scores a frame), because every run that a line's border cuts costs a
+    // line more: 131,072 x 2,000 f32 with next to nothing to multiply take 305 us in runs of 128 bytes and 214 us in runs of 1 KB.
+    // Two areas in turn: one barrier a pass.
+    //   held.j[FJ]: what column 32 c + (l & 31) of lane l's wave needs (lane_j); held.i[V]: what the lane's outputs need, those from
+    //   lane_i on.  pre(v, j, r): four sums on their way into LDS; post(v, i, j, r): outputs, j() = the column's held.j; out: a
+    //   TileOut.
+    template <class O> static __device__ __forceinline__ int lane_i() { return (threadIdx.x & 63) % (TI / RUN<O>) * RUN<O>; }
+    static __device__ __forceinline__ int lane_j(int c) { return (threadIdx.x >> 6) / WI * FJ * 32 + c * 32 + (threadIdx.x & 31); }
+
+    template <class O, class Held, class Pre, class Post, class Put>
+    static __device__ __forceinline__ void write_out(unsigned char *smem, const acc_t (&acc)[FI][FJ], const Held &held, Pre &&pre, Post &&post, Put &&out) {
+        constexpr int V = RUN<O>, ROW = TI * 4, COLS = 2 * WJ * 32 * ROW <= LDS ? 32 : 16, LPR = TI / V, RPI = 64 / LPR, EACH = COLS / WI;
+        static_assert(2 * WJ * COLS * ROW <= LDS && LPR <= 64 && EACH % RPI == 0 && EACH >= 1, "tile shape");
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        f32x4_t *st = reinterpret_cast<f32x4_t *>(smem + wave * (W * 32 * 4));
-        constexpr int MASK = (W / 4 < 32 ? W / 4 : 32) - 1;   // chunk c of row j at c ^ (j & MASK): no two lanes on one bank
-        const int h = lane >> 5, jw = lane & 31, ir = (lane % LPR) * V;
-        const auto held = begin((wave % WI) * W + ir);
+        const int wi = wave % WI, wj = wave / WI, h = lane >> 5, j = lane & 31;
 #pragma unroll
-        for (int f = 0; f < FJ; f++) {
+        for (int pass = 0; pass < FJ * 32 / COLS; pass++) {
+            const int c = pass * COLS / 32, from = pass * COLS % 32;
+            unsigned char *st = smem + ((pass & 1) * WJ + wj) * (COLS * ROW);
+            if (COLS == 32 || (j >= from && j < from + COLS)) {
 #pragma unroll
-            for (int i = 0; i < FI; i++)
+                for (int f = 0; f < FI; f++)
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const f32x4_t v = {(float)acc[i][f][4 * b], (float)acc[i][f][4 * b + 1], (float)acc[i][f][4 * b + 2], (float)acc[i][f][4 * b + 3]};
-                    st[jw * (W / 4) + ((i * 8 + b * 2 + h) ^ (jw & MASK))] = v;
-                }
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int r = 0; r < 32 / RPI; r++) {
-                const int j = r * RPI + lane / LPR;
-                float v[V];
-#pragma unroll
-                for (int q = 0; q < V / 4; q++) {
-                    const f32x4_t x = st[j * (W / 4) + ((ir / 4 + q) ^ (j & MASK))];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[4 * q + e] = x[e];
-                }
-                emit((wave % WI) * W + ir, (wave / WI) * FJ * 32 + f * 32 + j, v, held);
+                    for (int b = 0; b < 4; b++) {
+                        const acc_t &x = acc[f][c];
+                        const float v[4] = {(float)x[4 * b], (float)x[4 * b + 1], (float)x[4 * b + 2], (float)x[4 * b + 3]};
+                        f32x4_t r;
+                        pre(v, held.j[c], r);
+                        *reinterpret_cast<f32x4_t *>(st + (j - from) * ROW + (((wi * FI + f) * 8 + b * 2 + h) ^ (j & 7)) * 16) = r;
+                    }
             }
-            __builtin_amdgcn_wave_barrier();
+            if constexpr (WI > 1) lds_barrier(); else __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < EACH / RPI; q++) {
+                const int first = wi * EACH + q * RPI, col = first + lane / LPR;
+                float v[V], r[V];
+#pragma unroll
+                for (int e = 0; e < V / 4; e++) {
+                    const f32x4_t x = *reinterpret_cast<const f32x4_t *>(st + col * ROW + ((lane % LPR * (V / 4) + e) ^ ((from + col) & 7)) * 16);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) v[4 * e + d] = x[d];
+                }
+                post(v, held.i, [&]() { return from_lane(held.j[c], from + col); }, r);
+                out(wj * FJ * 32 + c * 32 + from + first, srx_pack<O, V>(r));
+            }
         }
     }
 };
 
-// Elements per 16-byte run of an output type
-template <class O>
-static constexpr int RUN = 16 / sizeof(O);
-
-// v to p[0 .. RUN), the first `n` of them; a whole run as one store, whatever its alignment
-template <class O>
-__device__ __forceinline__ void store_run(O *p, const float (&v)[RUN<O>], int64_t n) {
-    const typename SrxVec<O, RUN<O>>::type r = srx_pack<O, RUN<O>>(v);
-    if (n >= RUN<O>) __builtin_memcpy(p, &r, 16);
-    else
+// An output matrix, i adjacent: the tile that begins at (i = 0, j = 0) = base and of which ni x nj exist; TI / RUN lanes to a column.
+// Whole tiles go out without a look at each run's place, and every address is a scalar and the lane's 32-bit offset.
+// STREAM: past the caches, which the operands need (131,072 x 1,024 -> 2,048 f32 in 8 bits: 418 us through them, 366 us past them).
+template <class O, int TI, bool STREAM = true>
+struct TileOut {
+    static constexpr int V = RUN<O>, LPR = TI / V;
+    O *base;
+    int64_t ld;
+    int ni, nj;   // of the lane: outputs from its first i on, columns from its own on
+    bool whole;
+    unsigned lane;
+    __device__ __forceinline__ TileOut(O *b, int64_t ld_, int ni_, int nj_, bool whole_) : base(b), ld(ld_), whole(whole_) {
+        const int l = threadIdx.x & 63;
+        lane = (unsigned)(l / LPR * ld * (int64_t)sizeof(O)) + l % LPR * 16;
+        ni = ni_ - l % LPR * V;
+        nj = nj_ - l / LPR;
+    }
+    // (a run is stored whole whatever its alignment)
+    __device__ __forceinline__ void operator()(int j, const typename SrxVec<O, V>::type &r) const {
+        typedef int any_four __attribute__((ext_vector_type(4), aligned(2)));
+        char *p = reinterpret_cast<char *>(base + (int64_t)j * ld);
+        if (whole || (j < nj && ni >= V)) {
+            if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(any_four, r), reinterpret_cast<any_four *>(p + lane));
+            else __builtin_memcpy(p + lane, &r, 16);
+        } else if (j < nj && ni > 0) {
 #pragma unroll
-        for (int e = 0; e < RUN<O>; e++)
-            if (e < n) p[e] = r[e];
-}
+            for (int e = 0; e < V; e++)
+                if (e < ni) reinterpret_cast<O *>(p + lane)[e] = r[e];
+        }
+    }
+};
 
 // A tile of 32 x 32 for few rows, where the other operand is read once and nothing else costs: THIN_WAVES waves take the slabs in
 // turn, straight from memory into fragments (a wave's four k-steps use whole lines), two slabs in flight each, and add their
@@ -460,15 +504,16 @@ __device__ __forceinline__ void store_four(O *p, const float (&v)[4], int64_t n)
 
 // The tile (i, j) of workgroup b.  Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its own: an XCD gets a run
 // of neighbouring tiles, and the run goes through bands of TILE_BAND tiles of j, j first, so that the 32 tiles that its CUs hold at
-// a time are about 4 x 8 and read 12 operand slabs between them (in rows of i: 2 x 16 and 18).
-static constexpr int TILE_BAND = 8;
+// a time are about 4 x 8 and read 12 operand slabs between them (in rows of i: 2 x 16 and 18).  ni * nj < 2^31 / TILE_BAND.
+static constexpr unsigned TILE_BAND = 8;
 __device__ __forceinline__ void tile_of(int64_t b, int64_t ni, int64_t nj, int64_t &i, int64_t &j) {
-    const int64_t n = ni * nj, q = n / 8, r = n % 8, x = b % 8;
-    const int64_t item = x * q + (x < r ? x : r) + b / 8;
-    const int64_t band = item / (TILE_BAND * ni), in = item - band * (TILE_BAND * ni);
-    const int64_t h = nj - band * TILE_BAND < TILE_BAND ? nj - band * TILE_BAND : TILE_BAND;
-    i = in / h;
-    j = band * TILE_BAND + (in - i * h);
+    // (32 bits: a 64-bit division is a hundred instructions, and this stands between a workgroup's tiles)
+    const unsigned n = (unsigned)(ni * nj), q = n / 8, r = n % 8, x = (unsigned)b % 8;
+    const unsigned item = x * q + (x < r ? x : r) + (unsigned)b / 8, row = TILE_BAND * (unsigned)ni;
+    const unsigned band = item / row, in = item - band * row, left = (unsigned)nj - band * TILE_BAND;
+    const unsigned h = left < TILE_BAND ? left : TILE_BAND, ti = in / h;
+    i = ti;
+    j = band * TILE_BAND + (in - ti * h);
 }
 
 // Tile of 256 x 256 on 8 waves or of 128 x 128 on 4?  A CU holds one of the former or two of the latter.  A round of the small

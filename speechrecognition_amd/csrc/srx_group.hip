@@ -400,7 +400,7 @@ static int group_dw_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
 template <class El, class O>
 static int group_dw_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
     if (!tile_dma(p.x, p.ld_x, p.K, sizeof(El)) || !tile_dma(p.dy, p.ld_dy, p.N, sizeof(El))) return group_dw_tile<El, O, 2, 2, 2, 2, false>(ctx, name, p);
-    return dw_large(ctx, p.E, p.total, p.K, p.N) ? group_dw_tile<El, O, 2, 4, 4, 2, true>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, true>(ctx, name, p);
+    return dw_large(ctx, p.E, p.total, p.K, p.N) ? group_dw_tile<El, O, 4, 2, 2, 4, true>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, true>(ctx, name, p);
 }
 
 extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *x_dev, int64_t ld_x,

@@ -228,3 +228,62 @@ def test_refusals(ctx):
         a[i] = v
         assert lib.srx_group_matmul_dev(*a) == _capi.SRX_ERR_INVALID, (i, v)
     assert lib.srx_group_matmul_dw_scratch_bytes(h, 1, 1, 0, 1) == -1
+
+
+def _near(torch, got, want, mag, k, dtype):
+    """The bound of learned_ref.product and out_bound, on the GPU in 64 bits."""
+    err = R.U * (k + 1) * mag
+    return bool((torch.abs(got.double() - want) <= err + R.HALF[dtype] * (want.abs() + err) + R.TINY[dtype]).all())
+
+
+@pytest.mark.parametrize("dtype,pad", [("bf16", 0), ("f16", 5), ("f32", 0), ("bf16", 8)])
+def test_many_large_tiles(ctx, dtype, pad):
+    """Enough rows and columns for the 256 x 256 tiles (and, with odd strides, the 128 x 128 ones without direct loads): every
+    row and weight against the products in 64 bits."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(5)
+    lens, K, N = [9000, 0, 300, 20011, 3700], 136, 1032
+    off = np.concatenate([[0], np.cumsum(lens)])
+    T, E = int(off[-1]), len(lens)
+
+    def rand(r, c):
+        return torch.randn((r, c + pad), generator=g, device="cuda").to(_t(dtype))[:, :c]
+
+    x, dy = rand(T, K), rand(T, N)
+    w = torch.randn((E, N, K), generator=g, device="cuda").to(_t(dtype))
+    y, dx = torch.zeros((T, N), dtype=_t(dtype), device="cuda"), torch.zeros((T, K), dtype=_t(dtype), device="cuda")
+    dw, db = torch.zeros_like(w), torch.zeros((E, N), device="cuda")
+    offd = torch.from_numpy(off).cuda()
+    scratch = torch.full((max(host.group_matmul_dw_scratch_bytes(ctx, E, T, K, N), 16),), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    host.group_matmul(ctx, x, w, offd, y)
+    host.group_matmul_dx(ctx, dy, w, offd, dx)
+    host.group_matmul_dw(ctx, dy, x, offd, dw, dbias=db, scratch=scratch)
+    ctx.sync()
+    for e in range(E):
+        r = slice(int(off[e]), int(off[e + 1]))
+        X, D, W = x[r].double(), dy[r].double(), w[e].double()
+        assert _near(torch, y[r], X @ W.t(), X.abs() @ W.abs().t(), K, dtype), ("y", e)
+        assert _near(torch, dx[r], D @ W, D.abs() @ W.abs(), N, dtype), ("dx", e)
+        assert _near(torch, dw[e], D.t() @ X, D.abs().t() @ X.abs(), lens[e], dtype), ("dw", e)
+        assert _near(torch, db[e], D.sum(0), D.abs().sum(0), lens[e], "f32"), ("db", e)
+
+
+@pytest.mark.parametrize("lens", [[70000, 3, 0, 1], [1] * 500 + [40000]])
+def test_groups_of_very_different_sizes(ctx, lens):
+    """One group with nearly all rows: the others' dW are right beside it, wherever the shares fall."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(6)
+    K, N, T, E = 40, 72, sum(lens), len(lens)
+    off = np.concatenate([[0], np.cumsum(lens)])
+    x, dy = torch.randn((T, K), generator=g, device="cuda"), torch.randn((T, N), generator=g, device="cuda")
+    dw, db = torch.full((E, N, K), 5.0, device="cuda"), torch.full((E, N), 5.0, device="cuda")
+    offd = torch.from_numpy(off).cuda()
+    scratch = torch.full((max(host.group_matmul_dw_scratch_bytes(ctx, E, T, K, N), 16),), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    host.group_matmul_dw(ctx, dy, x, offd, dw, dbias=db, scratch=scratch)
+    ctx.sync()
+    for e in range(E):
+        D, X = dy[int(off[e]):int(off[e + 1])].double(), x[int(off[e]):int(off[e + 1])].double()
+        assert _near(torch, dw[e], D.t() @ X, D.abs().t() @ X.abs(), lens[e], "f32"), e
+        assert _near(torch, db[e], D.sum(0), D.abs().sum(0), lens[e], "f32"), e

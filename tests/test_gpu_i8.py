@@ -161,3 +161,22 @@ def test_refusals(ctx):
         a = list(ok)
         a[i] = v
         assert lib.srx_matmul_i8_dev(*a) == _capi.SRX_ERR_INVALID, (i, v)
+
+
+@pytest.mark.parametrize("out,by_state,pad", [("f32", False, 0), ("f32", True, 3), ("bf16", False, 1), ("f16", True, 0)])
+def test_many_large_tiles(ctx, out, by_state, pad):
+    """Enough scores for the 256 x 256 tiles, in both layouts, on lines of memory and off them."""
+    import torch
+    rows, N, K = 33011, 2000, 200
+    xq, xs, wq, ws, b = _operands(torch, rows, N, K, 3)
+    xs, ws = xs * 0.01, ws * 0.01
+    store = torch.full((N, rows + pad) if by_state else (rows, N + pad), 7.0, dtype=_t(out), device="cuda")
+    y = store.t()[:rows] if by_state else store[:, :N]
+    torch.cuda.synchronize()
+    host.matmul_i8(ctx, xq, xs, wq, ws, K, y, bias=b)
+    ctx.sync()
+    v = (xq[:, :K].double() @ wq[:, :K].double().t()) * xs.double()[:, None] * ws.double()
+    want = v + b.double()
+    err = 3.01 * R.U * v.abs() + R.U * want.abs()
+    assert (torch.abs(y.double() - want) <= err + R.HALF[out] * (want.abs() + err) + R.TINY[out]).all()
+    assert ((store[:, rows:] if by_state else store[:, N:]) == 7.0).all()

@@ -279,8 +279,13 @@ static int group_check(srx_ctx *ctx, const char *name, int in_dtype, int out_dty
     return SRX_OK;
 }
 
-// Rows of an average group up to which the forward product is bound by reading W once
+// 32 x 32 tiles: for groups of few rows on average (the product is bound by reading W once), and where even these tiles are no
+// more than the chip holds at a time (two to a CU): the larger ones would leave most of it idle, each with a long reduction
+// before it (345 rows x 1,370 -> 1 f32: 66 us as 3 tiles of 128 rows, 15 us as 11 of 32 with 8 waves to a reduction).
 static constexpr int64_t THIN_ROWS = 32;
+static bool group_thin(const srx_ctx *ctx, int64_t total, int E, int N) {
+    return total <= THIN_ROWS * E || (total / 32 + E) * ceil_div64(N, 32) <= 2 * (int64_t)ctx->num_cus;
+}
 
 template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, bool DMA>
 static int group_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
@@ -298,7 +303,7 @@ static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
     constexpr int Z = sizeof(El);
     const int I = DX ? p.K : p.N;
     if constexpr (!DX)
-        if (p.total <= THIN_ROWS * p.E) {
+        if (group_thin(ctx, p.total, p.E, p.N)) {
             p.tiles_i = ceil_div64(p.N, 32);
             p.tiles_j = p.total / 32 + p.E;
             SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);

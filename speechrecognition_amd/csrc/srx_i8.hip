@@ -240,7 +240,8 @@ extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev,
     return SRX_OK;
 }
 
-// Rows up to which the product is bound by reading the weights once
+// 32 x 32 tiles for few rows (the product is bound by reading the weights once), and where even these are no more than the chip
+// holds at a time
 static constexpr int64_t I8_THIN_ROWS = 64;
 
 template <class O, int WI, int WJ, int FI, int FJ>
@@ -256,7 +257,7 @@ static int i8_tile(srx_ctx *ctx, const char *name, I8Args &p) {
 
 template <class O>
 static int i8_launch(srx_ctx *ctx, const char *name, I8Args &p, int64_t rows) {
-    if (rows <= I8_THIN_ROWS) {
+    if (rows <= I8_THIN_ROWS || ceil_div64(p.I, 32) * ceil_div64(p.J, 32) <= 2 * (int64_t)ctx->num_cus) {
         p.tiles_i = ceil_div64(p.I, 32);
         p.tiles_j = ceil_div64(p.J, 32);
         SrxProf prof_(ctx, "k_matmul_i8_thin");

@@ -779,9 +779,9 @@ def quantize_rows(ctx, x, q, scale):
     return q, scale
 
 
-def matmul_i8(ctx, xq, xs, wq, ws, K, y, bias=None):
-    """y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n: codes xq [T][>= K], wq [N][>= K] int8, scales f32 -> y [T][N] (also a
-    transposed view: scores state by state)."""
+def matmul_i8(ctx, xq, xs, wq, ws, K, y, bias=None, by_state=False):
+    """y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n: codes xq [T][>= K], wq [N][>= K] int8, scales f32 -> y [T][N] (or a transposed
+    view of that shape); by_state: -> y [N][>= T], the rows that HmmBatch.viterbi reads fastest."""
     dev = ctx.device
     T, N, k16 = xq.shape[0], wq.shape[0], (K + 15) // 16 * 16
     if xq.shape[1] < k16:
@@ -791,15 +791,21 @@ def matmul_i8(ctx, xq, xs, wq, ws, K, y, bias=None):
     xp, ldx = _rows(xq, xq.shape, _I8, "xq", dev)
     wp, ldw = _rows(wq, wq.shape, _I8, "wq", dev)
     o = _one_of(_typed(y), "y", y)
-    if y.shape != (T, N) or y.get_device() != dev:
-        _refuse("y", y, f"[{T}][{N}] on device {dev}")
-    sr, sn = y.stride()
-    if sn == 1 or N == 1:
-        sr, sn = max(sr, N) if T == 1 else sr, 1
-    elif T == 1:
-        sr, sn = 1, max(sn, T)
+    if by_state:
+        if y.shape[0] != N or y.shape[1] < T:
+            _refuse("y", y, f"[{N}][{T}] on device {dev}")
+        yp, sn = _rows(y, y.shape, o, "y", dev)
+        sr = 1
+    else:
+        if y.shape != (T, N) or y.get_device() != dev:
+            _refuse("y", y, f"[{T}][{N}] on device {dev}")
+        yp, (sr, sn) = y.data_ptr(), y.stride()
+        if sn == 1 or N == 1:
+            sr, sn = max(sr, N) if T == 1 else sr, 1
+        elif T == 1:
+            sr, sn = 1, max(sn, T)
     rc = ctx.lib.srx_matmul_i8_dev(ctx.h, o, xp, ldx, _dense(xs, T, 0, "xs", dev), wp, ldw, _dense(ws, N, 0, "ws", dev), _dense(bias, N, 0, "bias", dev), T, N, K,
-                                   y.data_ptr(), sr, sn)
+                                   yp, sr, sn)
     if rc:
         check(rc, ctx.h)
     return y

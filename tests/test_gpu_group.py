@@ -287,3 +287,21 @@ def test_groups_of_very_different_sizes(ctx, lens):
         D, X = dy[int(off[e]):int(off[e + 1])].double(), x[int(off[e]):int(off[e + 1])].double()
         assert _near(torch, dw[e], D.t() @ X, D.abs().t() @ X.abs(), lens[e], "f32"), e
         assert _near(torch, db[e], D.sum(0), D.abs().sum(0), lens[e], "f32"), e
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+@pytest.mark.parametrize("lens,K,N", [([2600, 0, 77, 1900], 39, 264), ([2600, 0, 77, 1900], 136, 257), ([9000, 0, 33, 1500, 8000], 40, 41), ([5000, 4], 1, 130)])
+def test_more_small_tiles_than_the_chip_holds(ctx, dtype, out, pad, lens, K, N):
+    """Sizes whose forward product takes the 128-row tiles, wide and narrow, with and without direct loads."""
+    c = Case(ctx, lens, K, N, dtype, out, front=3, behind=70, pad=pad)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens,K,N", [([345], 1370, 1), ([800], 1000, 300), ([100, 0, 501, 3], 2056, 65)])
+def test_long_reductions_of_few_tiles(ctx, dtype, lens, K, N):
+    c = Case(ctx, lens, K, N, dtype, front=5, behind=9)
+    c.run()
+    c.check()

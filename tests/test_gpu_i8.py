@@ -180,3 +180,24 @@ def test_many_large_tiles(ctx, out, by_state, pad):
     err = 3.01 * R.U * v.abs() + R.U * want.abs()
     assert (torch.abs(y.double() - want) <= err + R.HALF[out] * (want.abs() + err) + R.TINY[out]).all()
     assert ((store[:, rows:] if by_state else store[:, N:]) == 7.0).all()
+
+
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("by_state", [False, True])
+@pytest.mark.parametrize("rows,N,K", [(700, 1003, 400), (2101, 260, 129), (5000, 33, 39), (300, 2001, 1025), (3000, 1025, 16)])
+def test_more_small_tiles_than_the_chip_holds(ctx, out, by_state, rows, N, K):
+    """Sizes that take the 128- and 256-row tiles, in odd numbers."""
+    import torch
+    xq, xs, wq, ws, b = _operands(torch, rows, N, K, rows + N + K)
+    xs, ws = (v * (0.01 if out == "f16" else 1) for v in (xs, ws))
+    store = torch.full((N, rows + 3) if by_state else (rows, N + 5), 7.0, dtype=_t(out), device="cuda")
+    torch.cuda.synchronize()
+    host.matmul_i8(ctx, xq, xs, wq, ws, K, store if by_state else store[:, :N], bias=b, by_state=by_state)
+    ctx.sync()
+    want = torch.from_numpy((xq.cpu().numpy()[:, :K].astype(np.float64) @ wq.cpu().numpy()[:, :K].T.astype(np.float64))).cuda()
+    want = want * xs.double()[:, None] * ws.double()
+    y = want + b.double()
+    err = 3.01 * R.U * want.abs() + R.U * y.abs()
+    got = (store.t()[:rows] if by_state else store[:, :N]).double()
+    assert bool(((got - y).abs() <= err + R.HALF[out] * (y.abs() + err) + R.TINY[out]).all())
+    assert bool(((store[:, rows:] if by_state else store[:, N:]) == 7.0).all())

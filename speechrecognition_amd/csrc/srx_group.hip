@@ -20,8 +20,11 @@ struct GroupArgs {
     int64_t total;
     int E, K, N;
     int64_t tiles_i, tiles_j;   // of the launch
-    float *part;                // dW's parts: two slots of TI * TJ + TJ floats per workgroup
+    float *part;                // dW's parts: two slots of TI * TJ + TJ floats per workgroup, and behind them a DwCut of each
 };
+
+// The tile that a workgroup of k_group_dw has begun and left to those after it, in `parts` parts with its own (0: it has not)
+struct alignas(16) DwCut { int e, i0, j0, parts; };
 
 __device__ __forceinline__ int64_t group_clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -51,9 +54,9 @@ __device__ __forceinline__ bool group_rows(const GroupArgs &p, int64_t t, int &e
 __device__ __forceinline__ void pass_four(const float (&v)[4], Nothing, f32x4_t &r) { r = {v[0], v[1], v[2], v[3]}; }
 
 // forward (DX false): i = output unit, reduction over K; dx: i = input unit, reduction over N, W read along its columns
-template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, bool DMA>
+template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, TileLoads HOW>
 __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group(GroupArgs p) {
-    typedef Tile<El, WI, WJ, FI, FJ, DX, false, DMA> T;
+    typedef Tile<El, WI, WJ, FI, FJ, DX, false, HOW> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
     struct Held {
         float i[RUN<O>];   // bias
@@ -71,8 +74,8 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group(GroupArgs p) {
     for (int q = 0; q < RUN<O>; q++) held.i[q] = !DX && p.bias && i + q < ni ? p.bias[(int64_t)e * p.N + i0 + i + q] : 0.0f;
     const El *w = reinterpret_cast<const El *>(p.w) + (int64_t)e * p.N * p.K;
     const int64_t ldq = DX ? p.ld_dy : p.ld_x;
-    const TileOperand P{DX ? w + i0 : w + (int64_t)i0 * p.K, p.K, ni};
-    const TileOperand Q{reinterpret_cast<const El *>(DX ? p.dy : p.x) + r0 * ldq, ldq, rows};
+    const TileOperand P{DX ? w + i0 : w + (int64_t)i0 * p.K, p.K, ni, i0};
+    const TileOperand Q{reinterpret_cast<const El *>(DX ? p.dy : p.x) + r0 * ldq, ldq, rows, 0};
     typename T::acc_t acc[FI][FJ];
     float none[FJ];
     T::template product<false>(smem, P, Q, DX ? p.N : p.K, acc, none, false);
@@ -85,6 +88,95 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group(GroupArgs p) {
         TileOut<O, T::TI>(reinterpret_cast<O *>(p.y) + r0 * p.ld_y + i0, p.ld_y, ni, rows, ni == T::TI && rows == T::TJ));
 }
 
+// Few outputs (up to 64) and a short reduction (up to NKS k-steps of 32 bytes): a transform of a frame's features.  W stays in a
+// wave's registers while it goes through SMALL_ROWS rows of the group, 32 at a time, straight from memory into fragments, the next
+// rows on their way behind the products; the outputs go out as they lie in the accumulators (the rows' lines are whole in L2).
+// No LDS and no barrier.
+static constexpr int SMALL_ROWS = 128, SMALL_OUT = 64, SMALL_BYTES = 256;
+
+template <class El, class O, bool DX, int NKS>
+__global__ __launch_bounds__(256, 2) void k_group_small(GroupArgs p) {
+#if defined(__HIP_DEVICE_COMPILE__)   // (the compiler's host pass does not know all of the builtins)
+    constexpr int Z = sizeof(El), EPC = 16 / Z;
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int e, rows;
+    int64_t r0;
+    if (!group_rows<SMALL_ROWS>(p, (int64_t)blockIdx.x * 4 + wave, e, r0, rows)) return;
+    constexpr unsigned OUTSIDE = 0x80000000u;
+    const int I = DX ? p.K : p.N, R = DX ? p.N : p.K, last = R % EPC ? R / EPC : -1;   // outputs; reduction; the chunk that its end cuts
+    const int64_t ldb = (DX ? p.ld_dy : p.ld_x) * Z;
+    const auto in = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(reinterpret_cast<const char *>(DX ? p.dy : p.x) + r0 * ldb), 0, (unsigned)((rows - 1) * ldb + R * Z), 0x00020000);
+    const auto wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<El *>(reinterpret_cast<const El *>(p.w) + (int64_t)e * p.N * p.K), 0, (unsigned)((int64_t)p.N * p.K * Z), 0x00020000);
+    // a chunk of a row at byte `row`: read in front of the row's end where that cuts it (then to be moved), zeros behind
+    auto run = [&](auto &from, unsigned row, int c) __attribute__((always_inline)) {
+        const int over = c * EPC + EPC - R;
+        return __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(from, over >= EPC ? OUTSIDE : row + c * 16 - (over > 0 ? over * Z : 0), 0, 0));
+    };
+    auto whole = [&](i32x4_t (&v)[NKS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ks = 0; ks < NKS; ks++)
+            if (last >> 1 == ks) v[ks] = drop_front(v[ks], ks * 2 + h == last ? (EPC - R % EPC) * Z : 0);   // (the same branch for all lanes)
+    };
+    i32x4_t w[2][NKS], x[NKS];
+#pragma unroll
+    for (int ks = 0; ks < NKS; ks++) x[ks] = run(in, (unsigned)((lane & 31) * ldb), ks * 2 + h);
+#pragma unroll
+    for (int f = 0; f < 2; f++) {
+        const int i = f * 32 + (lane & 31);
+#pragma unroll
+        for (int ks = 0; ks < NKS; ks++) {
+            if constexpr (!DX) w[f][ks] = run(wr, i < I ? (unsigned)(i * R * Z) : OUTSIDE, ks * 2 + h);
+            else {
+                El el[EPC];
+#pragma unroll
+                for (int q = 0; q < EPC; q++) {
+                    const int n = (ks * 2 + h) * EPC + q;
+                    const unsigned o = n < R && i < I ? (unsigned)((n * I + i) * Z) : OUTSIDE;
+                    if constexpr (Z == 4) el[q] = __builtin_bit_cast(El, __builtin_amdgcn_raw_buffer_load_b32(wr, o, 0, 0));
+                    else el[q] = __builtin_bit_cast(El, __builtin_amdgcn_raw_buffer_load_b16(wr, o, 0, 0));
+                }
+                __builtin_memcpy(&w[f][ks], el, 16);
+            }
+        }
+        if constexpr (!DX) whole(w[f]);
+    }
+    float bias[2][16];
+#pragma unroll
+    for (int f = 0; f < 2; f++)
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+            const int i = f * 32 + q / 4 * 8 + h * 4 + q % 4;
+            bias[f][q] = !DX && p.bias && i < I ? p.bias[(int64_t)e * I + i] : 0.0f;
+        }
+    O *out = reinterpret_cast<O *>(p.y) + r0 * p.ld_y;
+    for (int row = 0; row < rows; row += 32) {
+        i32x4_t next[NKS];
+#pragma unroll
+        for (int ks = 0; ks < NKS; ks++) next[ks] = run(in, (unsigned)((row + 32 + (lane & 31)) * ldb), ks * 2 + h);
+        whole(x);
+        const int j = row + (lane & 31);
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            typename MxType<El>::acc acc;
+#pragma unroll
+            for (int q = 0; q < 16; q++) acc[q] = 0;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ks++) MxType<El>::mma(acc, w[f][ks], x[ks]);
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const int i = f * 32 + b * 8 + h * 4;
+                float v[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) v[q] = acc[4 * b + q] + bias[f][4 * b + q];
+                if (j < rows && i < I) store_four<O>(out + (int64_t)j * p.ld_y + i, v, I - i);
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < NKS; ks++) x[ks] = next[ks];
+    }
+#endif
+}
+
 // forward, few rows per group: tiles of 32 x 32
 template <class El, class O>
 __global__ __launch_bounds__(THIN_WAVES * 64) void k_group_thin(GroupArgs p) {
@@ -94,8 +186,8 @@ __global__ __launch_bounds__(THIN_WAVES * 64) void k_group_thin(GroupArgs p) {
     int64_t r0;
     if (!group_rows<32>(p, blockIdx.x / p.tiles_i, e, r0, rows)) return;
     const El *w = reinterpret_cast<const El *>(p.w) + ((int64_t)e * p.N + i0) * p.K;
-    const TileOperand P{w, p.K, p.N - i0 < 32 ? p.N - i0 : 32};
-    const TileOperand Q{reinterpret_cast<const El *>(p.x) + r0 * p.ld_x, p.ld_x, rows};
+    const TileOperand P{w, p.K, p.N - i0 < 32 ? p.N - i0 : 32, 0};
+    const TileOperand Q{reinterpret_cast<const El *>(p.x) + r0 * p.ld_x, p.ld_x, rows, 0};
     O *y = reinterpret_cast<O *>(p.y);
     const float *bias = p.bias ? p.bias + (int64_t)e * p.N : nullptr;
     thin_product<El>(smem, P, Q, p.K, [&](int i, int j, const float (&v)[4]) {
@@ -163,9 +255,9 @@ __device__ __forceinline__ void dw_find(const GroupArgs &p, int64_t *sh, int64_t
     __syncthreads();
 }
 
-template <class El, class O, int WI, int WJ, int FI, int FJ, bool DMA>
+template <class El, class O, int WI, int WJ, int FI, int FJ, TileLoads HOW>
 __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group_dw(GroupArgs p) {
-    typedef Tile<El, WI, WJ, FI, FJ, true, true, DMA> T;
+    typedef Tile<El, WI, WJ, FI, FJ, true, true, HOW> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
     constexpr int64_t SLOT = T::TI * T::TJ + T::TJ;   // (whole lines: a multiple of 128 bytes)
     struct Held { Nothing i[1], j[FJ]; };
@@ -178,6 +270,7 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group_dw(GroupArgs p) {
     dw_find<T::KS, T::NT>(p, reinterpret_cast<int64_t *>(smem), tiles, me, G, total, len, e, before);
     int64_t at = me * len;
     const int64_t end = at + len < total ? at + len : total;
+    DwCut cut{0, 0, 0, 0};
     while (at < end) {
         int64_t n = dw_slabs<T::KS>(p, e);
         while (at >= (before + n) * tiles) {
@@ -191,8 +284,8 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group_dw(GroupArgs p) {
         const int64_t lo = a + s0 * T::KS < b ? a + s0 * T::KS : b, hi = a + s1 * T::KS < b ? a + s1 * T::KS : b;
         const int64_t tj = tile / p.tiles_i;
         const int i0 = (int)(tile - tj * p.tiles_i) * T::TI, j0 = (int)tj * T::TJ;
-        const TileOperand P{reinterpret_cast<const El *>(p.x) + lo * p.ld_x + i0, p.ld_x, p.K - i0 < T::TI ? p.K - i0 : T::TI};
-        const TileOperand Q{reinterpret_cast<const El *>(p.dy) + lo * p.ld_dy + j0, p.ld_dy, p.N - j0 < T::TJ ? p.N - j0 : T::TJ};
+        const TileOperand P{reinterpret_cast<const El *>(p.x) + lo * p.ld_x + i0, p.ld_x, p.K - i0 < T::TI ? p.K - i0 : T::TI, i0};
+        const TileOperand Q{reinterpret_cast<const El *>(p.dy) + lo * p.ld_dy + j0, p.ld_dy, p.N - j0 < T::TJ ? p.N - j0 : T::TJ, j0};
         const int slot = s0 > 0 ? 0 : s1 < n ? 1 : -1;   // -1: the whole reduction
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const bool wants = p.dbias != nullptr && i0 == 0 && wave % WI == 0;
@@ -200,6 +293,7 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group_dw(GroupArgs p) {
         float sums[FJ];
         T::template product<true>(smem, P, Q, hi - lo, acc, sums, wants);
         float *part = p.part + (me * 2 + (slot > 0)) * SLOT;
+        if (slot > 0) cut = {e, i0, j0, (int)(1 + (n - s1 + len - 1) / len)};
         if (wants) {
             const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -223,35 +317,29 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group_dw(GroupArgs p) {
         at += s1 - s0;
         lds_barrier();   // (the next product's loads go where columns were taken from)
     }
+    if (p.part && threadIdx.x == 0) reinterpret_cast<DwCut *>(p.part + G * 2 * SLOT)[me] = cut;
 }
 
-// Workgroup g of k_group_dw's G begins inside a tile: if it is the first to do so, this one adds the tile's parts -- slot 1 of the
-// workgroup before it, slot 0 of itself and of those that follow up to the tile's end.  blockIdx.y: JOIN_COLS of the tile's columns.
-static constexpr int JOIN_COLS = 8;
+// Adds the parts of the tile that workgroup blockIdx.x of k_group_dw's G has left to others: its slot 1, then slot 0 of those that
+// follow it.  blockIdx.y: as many of the tile's columns as 256 threads take in fours.
+template <int TI>
+static constexpr int JOIN_COLS = 1024 / TI;
 
-template <class O, int TI, int TJ, int KS>
+template <class O, int TI, int TJ>
 __global__ __launch_bounds__(256) void k_group_join(GroupArgs p, int64_t G) {
-    __shared__ int64_t sh[256];
     constexpr int64_t SLOT = TI * TJ + TJ;
-    const int64_t tiles = p.tiles_i * p.tiles_j, g = blockIdx.x + 1;
-    int64_t total, len, before;
-    int e;
-    dw_find<KS, 256>(p, sh, tiles, g, G, total, len, e, before);
-    const int64_t at = g * len;
-    if (at >= total) return;
-    const int64_t n = dw_slabs<KS>(p, e), tile = (at - before * tiles) / n, first = before * tiles + tile * n;
-    if (at == first || at - len > first) return;   // begins with the tile, or is not the first inside it
-    const int64_t parts = (first + n - 1) / len - g + 2;   // g - 1, g, .. the one that holds the tile's last slab
-    const int64_t tj = tile / p.tiles_i;
-    const int i0 = (int)(tile - tj * p.tiles_i) * TI, j0 = (int)tj * TJ;
-    const float *slot = p.part + ((g - 1) * 2 + 1) * SLOT;
-    constexpr int ROWS = JOIN_COLS;
+    const int64_t g = blockIdx.x;
+    const DwCut cut = reinterpret_cast<const DwCut *>(p.part + G * 2 * SLOT)[g];
+    if (cut.parts == 0) return;
+    const int e = cut.e, i0 = cut.i0, j0 = cut.j0, parts = cut.parts;
+    const float *slot = p.part + (g * 2 + 1) * SLOT;
+    constexpr int ROWS = JOIN_COLS<TI>;
     for (int c = threadIdx.x; c < ROWS * (TI / 4); c += 256) {
         const int j = blockIdx.y * ROWS + c / (TI / 4), i = c % (TI / 4) * 4;
         if (j0 + j >= p.N || i0 + i >= p.K) continue;
         f32x4_t v = *reinterpret_cast<const f32x4_t *>(slot + j * TI + i);
 #pragma unroll 4
-        for (int64_t q = 1; q < parts; q++) v += *reinterpret_cast<const f32x4_t *>(slot + (2 * q - 1) * SLOT + j * TI + i);
+        for (int q = 1; q < parts; q++) v += *reinterpret_cast<const f32x4_t *>(slot + (2 * q - 1) * SLOT + j * TI + i);
         const float f[4] = {v[0], v[1], v[2], v[3]};
         store_four<O>(reinterpret_cast<O *>(p.y) + ((int64_t)e * p.N + j0 + j) * p.K + i0 + i, f, p.K - i0 - i);
     }
@@ -259,7 +347,7 @@ __global__ __launch_bounds__(256) void k_group_join(GroupArgs p, int64_t G) {
         const int j = blockIdx.y * ROWS + threadIdx.x;
         if (j0 + j < p.N) {
             float v = slot[TI * TJ + j];
-            for (int64_t q = 1; q < parts; q++) v += slot[(2 * q - 1) * SLOT + TI * TJ + j];
+            for (int q = 1; q < parts; q++) v += slot[(2 * q - 1) * SLOT + TI * TJ + j];
             p.dbias[(int64_t)e * p.N + j0 + j] = v;
         }
     }
@@ -287,14 +375,23 @@ static bool group_thin(const srx_ctx *ctx, int64_t total, int E, int N) {
     return total <= THIN_ROWS * E || (total / 32 + E) * ceil_div64(N, 32) <= 2 * (int64_t)ctx->num_cus;
 }
 
-template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, bool DMA>
+template <class El, class O, bool DX, int WI, int WJ, int FI, int FJ, TileLoads HOW>
 static int group_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
-    typedef Tile<El, WI, WJ, FI, FJ, DX, false, DMA> T;
+    typedef Tile<El, WI, WJ, FI, FJ, DX, false, HOW> T;
     p.tiles_i = ceil_div64(DX ? p.K : p.N, T::TI);
     p.tiles_j = p.total / T::TJ + p.E;
     SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
     SrxProf prof_(ctx, DX ? "k_group_dx" : "k_group");
-    hipLaunchKernelGGL((k_group<El, O, DX, WI, WJ, FI, FJ, DMA>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
+    hipLaunchKernelGGL((k_group<El, O, DX, WI, WJ, FI, FJ, HOW>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
+    return SRX_OK;
+}
+
+template <class El, class O, bool DX, int NKS>
+static int group_small(srx_ctx *ctx, const char *name, GroupArgs &p) {
+    const int64_t blocks = ceil_div64(p.total / SMALL_ROWS + p.E, 4);
+    SRX_REQUIRE(ctx, blocks < (1ll << 28), "%s: too many tiles", name);
+    SrxProf prof_(ctx, DX ? "k_group_dx" : "k_group");
+    hipLaunchKernelGGL((k_group_small<El, O, DX, NKS>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
     return SRX_OK;
 }
 
@@ -303,7 +400,7 @@ static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
     constexpr int Z = sizeof(El);
     const int I = DX ? p.K : p.N;
     if constexpr (!DX)
-        if (group_thin(ctx, p.total, p.E, p.N)) {
+        if (p.K < 16 / Z || group_thin(ctx, p.total, p.E, p.N)) {
             p.tiles_i = ceil_div64(p.N, 32);
             p.tiles_j = p.total / 32 + p.E;
             SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
@@ -311,13 +408,22 @@ static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
             hipLaunchKernelGGL((k_group_thin<El, O>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(THIN_WAVES * 64), 0, ctx->stream, p);
             return SRX_OK;
         }
-    if (I <= 64) return group_tile<El, O, DX, 1, 4, 2, 1, false>(ctx, name, p);
+    if constexpr (DX)
+        if (p.N < 16 / Z || p.K < 16 / Z) return group_tile<El, O, DX, 2, 2, 2, 2, BY_ELEMENT>(ctx, name, p);
+    const int64_t bytes = (int64_t)(DX ? p.N : p.K) * Z;
+    if (I <= SMALL_OUT && bytes <= SMALL_BYTES) {
+        if (bytes <= 64) return group_small<El, O, DX, 2>(ctx, name, p);
+        if (bytes <= 128) return group_small<El, O, DX, 4>(ctx, name, p);
+        if (bytes <= 192) return group_small<El, O, DX, 6>(ctx, name, p);
+        return group_small<El, O, DX, 8>(ctx, name, p);
+    }
+    if (I <= 64) return group_tile<El, O, DX, 1, 4, 2, 1, BY_RUN>(ctx, name, p);
     // W is read along its columns (extent K) by dx, along its rows (K) by the forward product
     const bool dma = tile_dma(p.w, p.K, p.K, Z) && (DX ? tile_dma(p.dy, p.ld_dy, p.N, Z) : tile_dma(p.x, p.ld_x, p.K, Z));
-    if (!dma) return group_tile<El, O, DX, 2, 2, 2, 2, false>(ctx, name, p);
+    if (!dma) return group_tile<El, O, DX, 2, 2, 2, 2, BY_RUN>(ctx, name, p);
     if (tile_large(ceil_div64(I, 256) * (p.total / 256 + (p.E + 1) / 2), ceil_div64(I, 128) * (p.total / 128 + (p.E + 1) / 2), ctx->num_cus))
-        return group_tile<El, O, DX, 4, 2, 2, 4, true>(ctx, name, p);
-    return group_tile<El, O, DX, 2, 2, 2, 2, true>(ctx, name, p);
+        return group_tile<El, O, DX, 4, 2, 2, 4, TO_LDS>(ctx, name, p);
+    return group_tile<El, O, DX, 2, 2, 2, 2, TO_LDS>(ctx, name, p);
 }
 
 template <bool DX>
@@ -371,7 +477,7 @@ static int64_t dw_groups(const srx_ctx *ctx, int E, int64_t total, int K, int N,
     const int64_t g = ceil_div64(slabs, DW_SLABS);
     return g < 1 ? 1 : g < most ? g : most;
 }
-static int64_t dw_bytes(int64_t groups, int tile) { return groups < 2 ? 0 : groups * 2 * (tile * tile + tile) * (int64_t)sizeof(float); }
+static int64_t dw_bytes(int64_t groups, int tile) { return groups < 2 ? 0 : groups * (2 * (tile * tile + tile) * (int64_t)sizeof(float) + (int64_t)sizeof(DwCut)); }
 // 256 x 256 tiles where they cover no more than 128 x 128 ones do, and there is work for more than a slab or two each
 static bool dw_large(const srx_ctx *ctx, int E, int64_t total, int K, int N) {
     return ceil_div64(K, 256) * ceil_div64(N, 256) * 4 * 4 <= ceil_div64(K, 128) * ceil_div64(N, 128) * 5 &&
@@ -385,27 +491,29 @@ extern "C" int64_t srx_group_matmul_dw_scratch_bytes(const srx_ctx *ctx, int n_g
     return dw_large(ctx, n_groups, total_rows, K, N) && large > small ? large : small;   // (the larger slab counts of f32 bound the other types')
 }
 
-template <class El, class O, int WI, int WJ, int FI, int FJ, bool DMA>
+template <class El, class O, int WI, int WJ, int FI, int FJ, TileLoads HOW>
 static int group_dw_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
-    typedef Tile<El, WI, WJ, FI, FJ, true, true, DMA> T;
+    typedef Tile<El, WI, WJ, FI, FJ, true, true, HOW> T;
     p.tiles_i = ceil_div64(p.K, T::TI);
     p.tiles_j = ceil_div64(p.N, T::TJ);
     const int64_t G = dw_groups(ctx, p.E, p.total, p.K, p.N, T::TI, T::KS);
     {
         SrxProf prof_(ctx, "k_group_dw");
-        hipLaunchKernelGGL((k_group_dw<El, O, WI, WJ, FI, FJ, DMA>), dim3((unsigned)G), dim3(T::NT), 0, ctx->stream, p);
+        hipLaunchKernelGGL((k_group_dw<El, O, WI, WJ, FI, FJ, HOW>), dim3((unsigned)G), dim3(T::NT), 0, ctx->stream, p);
     }
     if (G > 1) {
         SrxProf prof_(ctx, "k_group_join");
-        hipLaunchKernelGGL((k_group_join<O, T::TI, T::TJ, T::KS>), dim3((unsigned)(G - 1), T::TJ / JOIN_COLS), dim3(256), 0, ctx->stream, p, G);
+        hipLaunchKernelGGL((k_group_join<O, T::TI, T::TJ>), dim3((unsigned)(G - 1), T::TJ / JOIN_COLS<T::TI>), dim3(256), 0, ctx->stream, p, G);
     }
     return SRX_OK;
 }
 
 template <class El, class O>
 static int group_dw_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
-    if (!tile_dma(p.x, p.ld_x, p.K, sizeof(El)) || !tile_dma(p.dy, p.ld_dy, p.N, sizeof(El))) return group_dw_tile<El, O, 2, 2, 2, 2, false>(ctx, name, p);
-    return dw_large(ctx, p.E, p.total, p.K, p.N) ? group_dw_tile<El, O, 4, 2, 2, 4, true>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, true>(ctx, name, p);
+    constexpr int Z = sizeof(El);
+    if (p.N < 16 / Z || p.K < 16 / Z) return group_dw_tile<El, O, 2, 2, 2, 2, BY_ELEMENT>(ctx, name, p);
+    if (!tile_dma(p.x, p.ld_x, p.K, Z) || !tile_dma(p.dy, p.ld_dy, p.N, Z)) return group_dw_tile<El, O, 2, 2, 2, 2, BY_RUN>(ctx, name, p);
+    return dw_large(ctx, p.E, p.total, p.K, p.N) ? group_dw_tile<El, O, 4, 2, 2, 4, TO_LDS>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, TO_LDS>(ctx, name, p);
 }
 
 extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *x_dev, int64_t ld_x,

@@ -142,15 +142,15 @@ __device__ __forceinline__ ScaleBias from_lane(const ScaleBias &v, int l) { retu
 
 template <class O, int WI, int WJ, int FI, int FJ>
 __global__ __launch_bounds__(WI *WJ * 64, 2) void k_matmul_i8(I8Args p) {
-    typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, true> T;
+    typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, TO_LDS> T;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[T::LDS];
     struct Held { ScaleBias i[RUN<O>], j[FJ]; };
     int64_t i0, j0;
     tile_of(blockIdx.x, p.tiles_i, p.tiles_j, i0, j0);
     i0 *= T::TI;
     j0 *= T::TJ;
-    const TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < T::TI ? p.I - i0 : T::TI)};
-    const TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < T::TJ ? p.J - j0 : T::TJ)};
+    const TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < T::TI ? p.I - i0 : T::TI), 0};
+    const TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < T::TJ ? p.J - j0 : T::TJ), 0};
     Held held;
     const int i = T::template lane_i<O>();
 #pragma unroll
@@ -182,8 +182,8 @@ template <class O>
 __global__ __launch_bounds__(THIN_WAVES * 64) void k_matmul_i8_thin(I8Args p) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[THIN_LDS];
     const int64_t i0 = (blockIdx.x % p.tiles_i) * 32, j0 = (blockIdx.x / p.tiles_i) * 32;
-    const TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < 32 ? p.I - i0 : 32)};
-    const TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < 32 ? p.J - j0 : 32)};
+    const TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < 32 ? p.I - i0 : 32), 0};
+    const TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < 32 ? p.J - j0 : 32), 0};
     O *y = reinterpret_cast<O *>(p.y);
     thin_product<int8_t>(smem, P, Q, (p.K + 15) / 16 * 16, [&](int i, int j, const float (&v)[4]) {
         if (j >= Q.n || i >= P.n) return;
@@ -246,7 +246,7 @@ static constexpr int64_t I8_THIN_ROWS = 64;
 
 template <class O, int WI, int WJ, int FI, int FJ>
 static int i8_tile(srx_ctx *ctx, const char *name, I8Args &p) {
-    typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, true> T;
+    typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, TO_LDS> T;
     p.tiles_i = ceil_div64(p.I, T::TI);
     p.tiles_j = ceil_div64(p.J, T::TJ);
     SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);

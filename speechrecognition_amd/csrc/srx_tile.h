@@ -56,90 +56,114 @@ template <> struct MxType<int8_t> {
     static __device__ __forceinline__ void mma(acc &c, i32x4_t p, i32x4_t q) { c = __builtin_amdgcn_mfma_i32_32x32x32_i8(p, q, c, 0, 0, 0); }
 };
 
-// An operand's part that a tile needs: `n` rows (or columns), element (0, k = 0) at base
+// An operand's part that a tile needs: `n` rows (or columns), element (0, k = 0) at base; columns: `before` more in front of it
 struct TileOperand {
     const void *base;
     int64_t ld;   // elements
-    int n;
+    int n, before;
 };
 
 typedef __attribute__((address_space(3))) unsigned char *lds_bytes;
 
 static constexpr int SLAB = 128, KSTEPS = SLAB / 32;
 
+// How 16-byte chunks come in.  TO_LDS: straight from memory, where every chunk is aligned and whole.  BY_RUN: through registers, any
+// address and extent of at least a chunk: the chunk that an extent's end cuts is read as the last 16 bytes in front of that end and
+// moved into place, so that every load is one instruction that is always issued (10,007 rows of 429 -> 500 f16, dx and dW: 21 and 23 us;
+// 32 and 31 where the last chunk comes element by element, in a branch; a second slab ahead in registers costs 5 to 15 % more).
+// BY_ELEMENT: extents below a chunk.
+enum TileLoads { BY_ELEMENT, BY_RUN, TO_LDS };
+
 // All loads of the wave have landed, all its LDS accesses are done, and so have everybody else's
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// v without its first `bytes` (0 .. 15, even), zeros behind
+__device__ __forceinline__ i32x4_t drop_front(i32x4_t v, int bytes) {
+    const bool two = bytes & 8, one = bytes & 4, half = bytes & 2;
+    v = two ? i32x4_t{v[2], v[3], 0, 0} : v;
+    v = one ? i32x4_t{v[1], v[2], v[3], 0} : v;
+    const uint32_t a = v[0], b = v[1], c = v[2], d = v[3];
+    return half ? i32x4_t{(int)(a >> 16 | b << 16), (int)(b >> 16 | c << 16), (int)(c >> 16 | d << 16), (int)(d >> 16)} : v;
+}
+
 // COLS: the operand's layout (see above); TX its extent in the tile; NT threads
-template <class El, bool COLS, int TX, int NT>
+template <class El, bool COLS, int TX, int NT, TileLoads HOW>
 struct TileLoader {
     static constexpr int Z = sizeof(El), EPC = 16 / Z, KS = SLAB / Z;     // elements per chunk, per slab
     static constexpr int CHUNKS = TX * SLAB / 16, PER = CHUNKS / NT;
     static constexpr int CPR = COLS ? TX * Z / 16 : SLAB / 16;            // chunks per slab row
-    static_assert(CHUNKS % NT == 0 && (!COLS || CPR >= 8), "tile shape");
+    static constexpr int STEP = NT / CPR;                                 // a thread's chunks: the same of every STEP-th slab row
+    static_assert(CHUNKS % NT == 0 && (!COLS || CPR >= 8) && NT % CPR == 0 && STEP % (COLS ? 4 : 8) == 0, "tile shape");
     static constexpr unsigned OUTSIDE = 0x80000000u;                      // past every bound: reads zeros
 
     const char *base;
     int64_t ldb;         // bytes per row of memory
-    int n;
+    int n, before;
     int64_t K;
-    unsigned off[PER];   // the chunk's byte offset from the slab's first row / column
-    int kin[PER];        // rows: first k of the chunk in its slab; columns: its k
-    int col[PER];        // rows: its row; columns: its first column
+    unsigned off, step;  // the first chunk's byte offset from the slab's first row / column; bytes to the next one
+    int kin;             // rows: first k of the chunks in the slab; columns: k of the first chunk
+    int col;             // rows: row of the first chunk; columns: first column of the chunks
 
     __device__ __forceinline__ void init(const TileOperand &o, int64_t K_, int t) {
-        base = reinterpret_cast<const char *>(o.base);
+        before = COLS && HOW == BY_RUN ? o.before : 0;   // (a chunk that is read from further left stays inside the descriptor)
+        base = reinterpret_cast<const char *>(o.base) - (int64_t)before * Z;
         ldb = o.ld * Z;
         n = o.n;
         K = K_;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int s = t + i * NT, r = s / CPR, cs = s % CPR;
-            if constexpr (COLS) {
-                const int c = cs ^ ((r & 3) << 1);
-                kin[i] = r;
-                col[i] = c * EPC;
-                off[i] = (unsigned)(r * ldb) + c * 16;
-                if (col[i] >= n) off[i] = OUTSIDE;
-            } else {
-                const int c = cs ^ (r & 7);
-                kin[i] = c * EPC;
-                col[i] = r;
-                off[i] = (unsigned)(r * ldb) + c * 16;
-            }
+        step = (unsigned)(STEP * ldb);
+        const int r = t / CPR, c = COLS ? t % CPR ^ ((r & 3) << 1) : t % CPR ^ (r & 7);
+        off = (unsigned)(r * ldb) + c * 16;
+        if constexpr (COLS) {
+            kin = r;
+            col = c * EPC;
+            off += before * Z;
+            if (col >= n) off = OUTSIDE;
+            else if (HOW == BY_RUN && col + EPC > n) off -= (col + EPC - n) * Z;
+        } else {
+            kin = c * EPC;
+            col = r;
         }
     }
-    // Straight into LDS, 16 bytes a lane, through a buffer descriptor whose bound makes everything outside the operand read
-    // as zeros.  Host's condition: base and ld are whole chunks, so is the extent along a chunk (n or K); a slab's span < 2 GiB.
-    struct Slab { __amdgpu_buffer_rsrc_t r; int64_t left; unsigned at; };
+    // A buffer descriptor whose bound makes everything outside the operand read as zeros.  Host's condition: a slab's span < 2 GiB.
+    struct Slab { __amdgpu_buffer_rsrc_t r; int left; unsigned at; };
     __device__ __forceinline__ Slab slab(int64_t k0) const {
         const int64_t left = K - k0;
         const char *b = COLS ? base + k0 * ldb : base;
         const int64_t rows = COLS ? (left < KS ? left : KS) : n;
-        const unsigned bound = rows > 0 ? (unsigned)((rows - 1) * ldb + (COLS ? (int64_t)n : K) * Z) : 0u;
-        return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(b), 0, bound, 0x00020000), left, COLS ? 0u : (unsigned)(k0 * Z)};
+        const unsigned bound = rows > 0 ? (unsigned)((rows - 1) * ldb + (COLS ? (int64_t)(before + n) : K) * Z) : 0u;
+        return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(b), 0, bound, 0x00020000), left < 0 ? 0 : left < KS ? (int)left : KS, COLS ? 0u : (unsigned)(k0 * Z)};
     }
+    // Host's condition: base and ld are whole chunks, and so is the extent along a chunk (n or K)
     __device__ __forceinline__ void dma(const Slab &s, int i, lds_bytes dst, int wave) const {
-        const unsigned o = COLS ? off[i] : kin[i] < s.left ? off[i] + s.at : OUTSIDE;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(s.r, (__attribute__((address_space(3))) void *)(dst + (i * NT + wave * 64) * 16), 16, o, 0, 0, 0);
+        const unsigned o = COLS ? off : kin < s.left ? off + s.at : OUTSIDE;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(s.r, (__attribute__((address_space(3))) void *)(dst + (i * NT + wave * 64) * 16), 16, o + i * step, 0, 0, 0);
     }
-    // Any alignment and size: whole chunks by one (unaligned) 16-byte load, the rest element by element
-    __device__ __forceinline__ void load(int64_t k0, i32x4_t (&v)[PER]) const {
-        const char *b = base + k0 * (COLS ? ldb : Z);
+    // BY_RUN.  Host's condition: the extent along a chunk is no less than one (columns: with those in front)
+    __device__ __forceinline__ void load(const Slab &s, i32x4_t (&v)[PER]) const {
+        const int over = kin + EPC - s.left;
+        const unsigned o = COLS ? off : over >= EPC ? OUTSIDE : off + s.at - (over > 0 ? over * Z : 0);
+#pragma unroll
+        for (int i = 0; i < PER; i++) v[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(s.r, o + i * step, 0, 0));
+    }
+    __device__ __forceinline__ void place(int64_t k0, i32x4_t (&v)[PER]) const {
+        const int64_t left = K - k0;
+        if (COLS ? n % EPC != 0 : left > 0 && left < KS && left % EPC != 0) {   // (the same for all lanes)
+            const int over = COLS ? col + EPC - n : kin + EPC - (int)left;
+#pragma unroll
+            for (int i = 0; i < PER; i++) v[i] = drop_front(v[i], over > 0 && over < EPC ? over * Z : 0);
+        }
+    }
+    // BY_ELEMENT: any size
+    __device__ __forceinline__ void load_elements(int64_t k0, i32x4_t (&v)[PER]) const {
+        const El *p = reinterpret_cast<const El *>(base + k0 * (COLS ? ldb : Z) + off);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int64_t left = K - k0 - kin[i];
-            const int64_t have = COLS ? (left > 0 ? n - col[i] : 0) : (col[i] < n ? left : 0);
-            const char *p = b + off[i];   // (only where have > 0)
-            i32x4_t r = {0, 0, 0, 0};
-            if (have >= EPC) __builtin_memcpy(&r, p, 16);
-            else if (have > 0) {
-                El e[EPC];
+            const int64_t left = K - k0 - kin - (COLS ? i * STEP : 0);
+            const int64_t have = COLS ? (left > 0 ? n - col : 0) : (col + i * STEP < n ? left : 0);
+            El e[EPC];
 #pragma unroll
-                for (int q = 0; q < EPC; q++) e[q] = q < have ? reinterpret_cast<const El *>(p)[q] : (El)0;
-                __builtin_memcpy(&r, e, 16);
-            }
-            v[i] = r;
+            for (int q = 0; q < EPC; q++) e[q] = q < have ? p[(int64_t)i * STEP * ldb / Z + q] : (El)0;
+            __builtin_memcpy(&v[i], e, 16);
         }
     }
     __device__ __forceinline__ void store(const i32x4_t (&v)[PER], lds_bytes dst, int t) const {
@@ -197,9 +221,10 @@ __device__ __forceinline__ float from_lane(float v, int l) { return __shfl(v, l)
 struct Nothing {};
 __device__ __forceinline__ Nothing from_lane(Nothing, int) { return {}; }
 
-// WI x WJ waves of FI x FJ fragments of 32 x 32.  DMA: see TileLoader::slab for what the host has to have checked.
-template <class El, int WI_, int WJ_, int FI_, int FJ_, bool PC, bool QC, bool DMA>
+// WI x WJ waves of FI x FJ fragments of 32 x 32.  HOW: see TileLoader for what the host has to have checked.
+template <class El, int WI_, int WJ_, int FI_, int FJ_, bool PC, bool QC, TileLoads HOW>
 struct Tile {
+    static constexpr bool DMA = HOW == TO_LDS;
     static constexpr int WI = WI_, WJ = WJ_, FI = FI_, FJ = FJ_;
     static constexpr int NT = WI * WJ * 64, TI = WI * FI * 32, TJ = WJ * FJ * 32;
     static constexpr int KS = SLAB / sizeof(El);
@@ -215,8 +240,8 @@ struct Tile {
         const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
         const int wi = wave % WI, wj = wave / WI;
         const lds_bytes lds = (lds_bytes)smem;
-        TileLoader<El, PC, TI, NT> lp;
-        TileLoader<El, QC, TJ, NT> lq;
+        TileLoader<El, PC, TI, NT, HOW> lp;
+        TileLoader<El, QC, TJ, NT, HOW> lq;
         TileReader<El, PC, TI> rp;
         TileReader<El, QC, TJ> rq;
         rp.init(wi * FI * 32, lane);
@@ -225,25 +250,32 @@ struct Tile {
         // registers).  Fragments are read one k-step ahead of their products; the barrier at a slab's end stands before its last
         // k-step's products, when everything of the slab has been read, so that the next slab's first fragments and the loads of
         // the slab after that one go out behind it.
-        constexpr int EACH = TileLoader<El, PC, TI, NT>::PER + TileLoader<El, QC, TJ, NT>::PER;
+        constexpr int EACH = TileLoader<El, PC, TI, NT, HOW>::PER + TileLoader<El, QC, TJ, NT, HOW>::PER;
         i32x4_t vp[DMA ? 1 : lp.PER], vq[DMA ? 1 : lq.PER];
         auto ahead = [&](int64_t s, int stage) __attribute__((always_inline)) {
-            const lds_bytes to = lds + stage * STAGE;
             if constexpr (DMA) {
+                const lds_bytes to = lds + stage * STAGE;
                 const auto sp = lp.slab(s * KS);
                 const auto sq = lq.slab(s * KS);
 #pragma unroll
                 for (int i = 0; i < lp.PER; i++) lp.dma(sp, i, to, wave);
 #pragma unroll
                 for (int i = 0; i < lq.PER; i++) lq.dma(sq, i, to + TI * SLAB, wave);
+            } else if constexpr (HOW == BY_RUN) {
+                lp.load(lp.slab(s * KS), vp);
+                lq.load(lq.slab(s * KS), vq);
             } else {
-                lp.load(s * KS, vp);
-                lq.load(s * KS, vq);
+                lp.load_elements(s * KS, vp);
+                lq.load_elements(s * KS, vq);
             }
         };
-        auto settle = [&](int stage) __attribute__((always_inline)) {   // registers into LDS
+        auto settle = [&](int64_t s, int stage) __attribute__((always_inline)) {   // registers into LDS
             if constexpr (!DMA) {
                 const lds_bytes to = lds + stage * STAGE;
+                if constexpr (HOW == BY_RUN) {
+                    lp.place(s * KS, vp);
+                    lq.place(s * KS, vq);
+                }
                 lp.store(vp, to, t);
                 lq.store(vq, to + TI * SLAB, t);
             }
@@ -288,8 +320,8 @@ struct Tile {
                 for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
 #pragma unroll
         for (int j = 0; j < FJ; j++) sums[j] = 0.0f;
-        settle(0);
-        tile_barrier();
+        settle(0, 0);
+        if constexpr (DMA) tile_barrier(); else lds_barrier();
         if constexpr (!DMA) ahead(1, 1);
         fetch(0, 0, 0);
         for (int64_t s = 0; s < slabs; s++) {
@@ -302,8 +334,8 @@ struct Tile {
                 __builtin_amdgcn_sched_barrier(0);
             }
             // (behind the last slab all this goes on with zeros, which nobody uses: one path for the accumulators)
-            settle(nxt);
-            tile_barrier();
+            settle(s + 1, nxt);
+            if constexpr (DMA) tile_barrier(); else lds_barrier();   // (loads into registers stay on their way)
             fetch(nxt, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (DMA) {

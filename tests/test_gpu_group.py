@@ -305,3 +305,11 @@ def test_long_reductions_of_few_tiles(ctx, dtype, lens, K, N):
     c = Case(ctx, lens, K, N, dtype, front=5, behind=9)
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("K,N,pad", [(39, 39, 0), (39, 13, 1), (8, 3, 0), (16, 64, 0), (33, 7, 3), (64, 64, 0), (64, 1, 8), (100, 50, 0), (13, 60, 4), (128, 33, 0)])
+def test_small_weights_and_many_rows(ctx, dtype, out, K, N, pad):
+    c = Case(ctx, [9000, 0, 1, 129, 10001, 128, 1900], K, N, dtype, out, front=7, behind=200, pad=pad)
+    c.run()
+    c.check()

@@ -91,8 +91,9 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_group(GroupArgs p) {
 // Few outputs (up to 64) and a short reduction (up to NKS k-steps of 32 bytes): a transform of a frame's features.  W stays in a
 // wave's registers while it goes through SMALL_ROWS rows of the group, 32 at a time, straight from memory into fragments, the next
 // rows on their way behind the products; the outputs go out as they lie in the accumulators (the rows' lines are whole in L2).
-// No LDS and no barrier.
-static constexpr int SMALL_ROWS = 128, SMALL_OUT = 64, SMALL_BYTES = 256;
+// No LDS and no barrier.  1,000 speakers, 499,674 rows of 39 -> 39 f32 (156 MB): 56 us; 81 us through LDS tiles of 64 x 128, 61 and 64 us
+// with 128 and 256 rows to a wave.
+static constexpr int SMALL_ROWS = 64, SMALL_OUT = 64, SMALL_BYTES = 256;
 
 template <class El, class O, bool DX, int NKS>
 __global__ __launch_bounds__(256, 2) void k_group_small(GroupArgs p) {
@@ -445,7 +446,8 @@ extern "C" int srx_group_matmul_dev(srx_ctx *ctx, int in_dtype, int out_dtype, c
     if (rc != SRX_OK || n_groups == 0 || total_rows == 0) return rc;
     SRX_REQUIRE(ctx, x_dev && w_dev && row_off_dev && y_dev, "%s: null argument", name);
     SRX_REQUIRE(ctx, ld_x >= K && ld_y >= N && ld_x <= GROUP_MAX_LD && ld_y <= GROUP_MAX_LD, "%s: row strides %lld, %lld for %d / %d columns", name, (long long)ld_x, (long long)ld_y, K, N);
-    SRX_REQUIRE(ctx, srx_aligned(x_dev, srx_dtype_size(in_dtype)) && srx_aligned(w_dev, srx_dtype_size(in_dtype)) && srx_aligned(y_dev, srx_dtype_size(out_dtype)),
+    SRX_REQUIRE(ctx, srx_aligned(x_dev, srx_dtype_size(in_dtype)) && srx_aligned(w_dev, srx_dtype_size(in_dtype)) && srx_aligned(y_dev, srx_dtype_size(out_dtype)) &&
+                         srx_aligned(bias_dev, 4) && srx_aligned(row_off_dev, 8),
                 "%s: misaligned buffer", name);
     GroupArgs p{};
     p.x = x_dev; p.ld_x = ld_x; p.w = w_dev; p.bias = bias_dev; p.y = y_dev; p.ld_y = ld_y;
@@ -461,7 +463,8 @@ extern "C" int srx_group_matmul_dx_dev(srx_ctx *ctx, int in_dtype, int out_dtype
     if (rc != SRX_OK || n_groups == 0 || total_rows == 0) return rc;
     SRX_REQUIRE(ctx, dy_dev && w_dev && row_off_dev && dx_dev, "%s: null argument", name);
     SRX_REQUIRE(ctx, ld_dy >= N && ld_dx >= K && ld_dy <= GROUP_MAX_LD && ld_dx <= GROUP_MAX_LD, "%s: row strides %lld, %lld for %d / %d columns", name, (long long)ld_dy, (long long)ld_dx, N, K);
-    SRX_REQUIRE(ctx, srx_aligned(dy_dev, srx_dtype_size(in_dtype)) && srx_aligned(w_dev, srx_dtype_size(in_dtype)) && srx_aligned(dx_dev, srx_dtype_size(out_dtype)),
+    SRX_REQUIRE(ctx, srx_aligned(dy_dev, srx_dtype_size(in_dtype)) && srx_aligned(w_dev, srx_dtype_size(in_dtype)) && srx_aligned(dx_dev, srx_dtype_size(out_dtype)) &&
+                         srx_aligned(row_off_dev, 8),
                 "%s: misaligned buffer", name);
     GroupArgs p{};
     p.dy = dy_dev; p.ld_dy = ld_dy; p.w = w_dev; p.y = dx_dev; p.ld_y = ld_dx;
@@ -525,7 +528,8 @@ extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype
     if (rc != SRX_OK || n_groups == 0) return rc;
     SRX_REQUIRE(ctx, row_off_dev && dw_dev && (total_rows == 0 || (dy_dev && x_dev)), "%s: null argument", name);
     SRX_REQUIRE(ctx, ld_dy >= N && ld_x >= K && ld_dy <= GROUP_MAX_LD && ld_x <= GROUP_MAX_LD, "%s: row strides %lld, %lld for %d / %d columns", name, (long long)ld_dy, (long long)ld_x, N, K);
-    SRX_REQUIRE(ctx, srx_aligned(dy_dev, srx_dtype_size(in_dtype)) && srx_aligned(x_dev, srx_dtype_size(in_dtype)) && srx_aligned(dw_dev, srx_dtype_size(out_dtype)),
+    SRX_REQUIRE(ctx, srx_aligned(dy_dev, srx_dtype_size(in_dtype)) && srx_aligned(x_dev, srx_dtype_size(in_dtype)) && srx_aligned(dw_dev, srx_dtype_size(out_dtype)) &&
+                         srx_aligned(dbias_dev, 4) && srx_aligned(row_off_dev, 8),
                 "%s: misaligned buffer", name);
     GroupArgs p{};
     p.dy = dy_dev; p.ld_dy = ld_dy; p.x = x_dev; p.ld_x = ld_x; p.y = dw_dev; p.dbias = dbias_dev;

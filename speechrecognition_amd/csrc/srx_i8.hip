@@ -283,7 +283,7 @@ extern "C" int srx_matmul_i8_dev(srx_ctx *ctx, int out_dtype, const int8_t *xq_d
                 "%s: code rows of %lld / %lld bytes for K = %d (whole 16 bytes, 16-byte aligned, at most 4 MiB)", name, (long long)ld_xq, (long long)ld_wq, K);
     SRX_REQUIRE(ctx, (stride_n == 1 && stride_r >= N && stride_r <= (1 << 26)) || (stride_r == 1 && stride_n >= rows && stride_n <= (1 << 26)), "%s: output strides %lld, %lld (one of them 1, the other at most 2^26 and no less than what it crosses)", name, (long long)stride_r,
                 (long long)stride_n);
-    SRX_REQUIRE(ctx, srx_aligned(y_dev, srx_dtype_size(out_dtype)), "%s: misaligned buffer", name);
+    SRX_REQUIRE(ctx, srx_aligned(y_dev, srx_dtype_size(out_dtype)) && srx_aligned(xs_dev, 4) && srx_aligned(ws_dev, 4) && srx_aligned(bias_dev, 4), "%s: misaligned buffer", name);
     I8Args p{};
     p.K = K;
     p.bias = bias_dev;

@@ -529,7 +529,9 @@ extern "C" int srx_gated_scan_dev(srx_ctx *ctx, int mode, int dtype, const void 
     SRX_REQUIRE(ctx, frame_off_dev && (total_frames == 0 || (gate_dev && x_dev && h_dev)), "%s: null argument", name);
     SRX_REQUIRE(ctx, ld_gate >= D && ld_x >= D && ld_h >= D, "%s: a row stride below %d channels", name, D);
     const size_t z = srx_dtype_size(dtype);
-    SRX_REQUIRE(ctx, srx_aligned(gate_dev, z) && srx_aligned(x_dev, z) && srx_aligned(h_dev, z), "%s: misaligned buffer", name);
+    SRX_REQUIRE(ctx, srx_aligned(gate_dev, z) && srx_aligned(x_dev, z) && srx_aligned(h_dev, z) && srx_aligned(h0_dev, 4) && srx_aligned(h_last_dev, 4) && srx_aligned(states_dev, 4) &&
+                         srx_aligned(frame_off_dev, 8),
+                "%s: misaligned buffer", name);
     ScanArgs p{};
     p.gate = gate_dev; p.ld_gate = ld_gate;
     p.x = x_dev; p.ld_x = ld_x;
@@ -552,7 +554,8 @@ extern "C" int srx_gated_scan_backward_dev(srx_ctx *ctx, int mode, int dtype, co
     SRX_REQUIRE(ctx, frame_off_dev && (total_frames == 0 || (gate_dev && x_dev && states_dev && dh_dev && dgate_dev && dx_dev)), "%s: null argument", name);
     SRX_REQUIRE(ctx, ld_gate >= D && ld_x >= D && ld_dh >= D && ld_dgate >= D && ld_dx >= D, "%s: a row stride below %d channels", name, D);
     const size_t z = srx_dtype_size(dtype);
-    SRX_REQUIRE(ctx, srx_aligned(gate_dev, z) && srx_aligned(x_dev, z) && srx_aligned(dh_dev, z) && srx_aligned(dgate_dev, z) && srx_aligned(dx_dev, z),
+    SRX_REQUIRE(ctx, srx_aligned(gate_dev, z) && srx_aligned(x_dev, z) && srx_aligned(dh_dev, z) && srx_aligned(dgate_dev, z) && srx_aligned(dx_dev, z) &&
+                         srx_aligned(states_dev, 4) && srx_aligned(dh_last_dev, 4) && srx_aligned(dh0_dev, 4) && srx_aligned(frame_off_dev, 8),
                 "%s: misaligned buffer", name);
     ScanArgs p{};
     p.gate = gate_dev; p.ld_gate = ld_gate;

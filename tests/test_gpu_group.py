@@ -313,3 +313,14 @@ def test_small_weights_and_many_rows(ctx, dtype, out, K, N, pad):
     c = Case(ctx, [9000, 0, 1, 129, 10001, 128, 1900], K, N, dtype, out, front=7, behind=200, pad=pad)
     c.run()
     c.check()
+
+
+def test_misaligned_tables_are_refused(ctx):
+    c = Case(ctx, [20, 30], 24, 40, "bf16")
+    lib, h = ctx.lib, ctx.h
+    x, w, b, o, y, dy, dx, dw, db = (v.data_ptr() for v in (c.x, c.w, c.bias, c.offd, c.y, c.dy, c.dx, c.dw, c.db))
+    s = (c.scratch.data_ptr(), c.scratch.numel())
+    for bias, off in ((b + 2, o), (b, o + 4)):
+        assert lib.srx_group_matmul_dev(h, 2, 2, x, 24, w, bias, off, 2, 50, 24, 40, y, 40) == _capi.SRX_ERR_INVALID
+        assert lib.srx_group_matmul_dw_dev(h, 2, 2, dy, 40, x, 24, off, 2, 50, 24, 40, dw, db + bias - b, *s) == _capi.SRX_ERR_INVALID
+    assert lib.srx_group_matmul_dx_dev(h, 2, 2, dy, 40, w, o + 4, 2, 50, 24, 40, dx, 24) == _capi.SRX_ERR_INVALID

@@ -201,3 +201,12 @@ def test_more_small_tiles_than_the_chip_holds(ctx, out, by_state, rows, N, K):
     got = (store.t()[:rows] if by_state else store[:, :N]).double()
     assert bool(((got - y).abs() <= err + R.HALF[out] * (y.abs() + err) + R.TINY[out]).all())
     assert bool(((store[:, rows:] if by_state else store[:, N:]) == 7.0).all())
+
+
+def test_misaligned_scales_are_refused(ctx):
+    import torch
+    xq, xs, wq, ws, b = _operands(torch, 4, 20, 40, 0)
+    y = torch.zeros((4, 20), device="cuda")
+    for i in range(3):
+        p = [v.data_ptr() + (2 if k == i else 0) for k, v in enumerate((xs, ws, b))]
+        assert ctx.lib.srx_matmul_i8_dev(ctx.h, 0, xq.data_ptr(), 48, p[0], wq.data_ptr(), 48, p[1], p[2], 4, 20, 40, y.data_ptr(), 20, 1) == _capi.SRX_ERR_INVALID

@@ -11,9 +11,11 @@
 // the operand layout of v_mfma 32x32x16 (16 bit) and 32x32x32 (8 bit).  f32 runs four 32x32x2 on the chunk's four elements; any
 // order of k is right as long as both operands have the same.
 //
-// Rows slab: chunk c of row r at r * 128 + ((c ^ (r & 7)) << 4): eight neighbouring rows' chunks lie on eight different bank
-// groups.  Columns slab: [k][TX] with the column's 32-byte pairs moved by (k & 3): 16-bit fragments come through
-// ds_read_b64_tr_b16 (each group of 16 lanes reads 4 k x 16 columns and gets them transposed), f32 ones element by element.
+// Bank conflicts: LDS has 64 banks of 4 bytes and serves 256 bytes, 16 lanes of a 16-byte read, together.  Rows slab: chunk c of row r
+// at r * 128 + ((c ^ (r >> 1 & 7)) << 4): 16 neighbouring rows' chunks cover all banks.  Columns slab: [k][TX]; 16-bit fragments come
+// through ds_read_b64_tr_b16 (each group of 16 lanes reads 4 k x 16 columns and gets them transposed), 32 lanes 4 k x 64 bytes
+// together, so the columns' 64-byte parts are moved by k & 3; f32 ones come element by element, both half-waves' k together, so
+// their 128-byte parts are moved by bit 2 of k (turned()).
 //
 // Result layout: lane l holds column j = l & 31, rows 8 b + 4 (l >> 5) + 0..3 for b = 0..3: four adjacent i for one j.
 #pragma once
@@ -86,6 +88,13 @@ __device__ __forceinline__ i32x4_t drop_front(i32x4_t v, int bytes) {
     return half ? i32x4_t{(int)(a >> 16 | b << 16), (int)(b >> 16 | c << 16), (int)(c >> 16 | d << 16), (int)(d >> 16)} : v;
 }
 
+// Columns slab: the column chunk that lies at chunk c of row k (and the other way round)
+template <class El, int TX>
+__device__ __forceinline__ int turned(int k, int c) {
+    if (sizeof(El) == 4) return c ^ ((k >> 2 & 1) << 3);
+    return TX >= 128 ? c ^ ((k & 3) << 2) : c ^ ((k >> 1 & 1) << 2);   // (64 columns: two rows to 256 bytes)
+}
+
 // COLS: the operand's layout (see above); TX its extent in the tile; NT threads
 template <class El, bool COLS, int TX, int NT, TileLoads HOW>
 struct TileLoader {
@@ -93,7 +102,7 @@ struct TileLoader {
     static constexpr int CHUNKS = TX * SLAB / 16, PER = CHUNKS / NT;
     static constexpr int CPR = COLS ? TX * Z / 16 : SLAB / 16;            // chunks per slab row
     static constexpr int STEP = NT / CPR;                                 // a thread's chunks: the same of every STEP-th slab row
-    static_assert(CHUNKS % NT == 0 && (!COLS || CPR >= 8) && NT % CPR == 0 && STEP % (COLS ? 4 : 8) == 0, "tile shape");
+    static_assert(CHUNKS % NT == 0 && (!COLS || CPR >= 8) && NT % CPR == 0 && STEP % (COLS ? 8 : 16) == 0, "tile shape");
     static constexpr unsigned OUTSIDE = 0x80000000u;                      // past every bound: reads zeros
 
     const char *base;
@@ -111,7 +120,7 @@ struct TileLoader {
         n = o.n;
         K = K_;
         step = (unsigned)(STEP * ldb);
-        const int r = t / CPR, c = COLS ? t % CPR ^ ((r & 3) << 1) : t % CPR ^ (r & 7);
+        const int r = t / CPR, c = COLS ? turned<El, TX>(r, t % CPR) : t % CPR ^ (r >> 1 & 7);
         off = (unsigned)(r * ldb) + c * 16;
         if constexpr (COLS) {
             kin = r;
@@ -177,20 +186,19 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // A lane's fragments of one operand, `first`: the wave's first row / column in the tile
 template <class El, bool COLS, int TX>
 struct TileReader {
-    unsigned at[4];   // rows: by k-step; columns: by parity of the fragment (16 bit), by element (f32)
+    unsigned at[4];   // rows: by k-step; columns: by fragment
     __device__ __forceinline__ void init(int first, int lane) {
-        const int h = lane >> 5;
+        const int h = lane >> 5, l = lane & 31;
         if constexpr (!COLS) {
 #pragma unroll
-            for (int ks = 0; ks < KSTEPS; ks++) at[ks] = (first + (lane & 31)) * SLAB + (((ks * 2 + h) ^ (lane & 7)) << 4);
-        } else if constexpr (sizeof(El) == 2) {
-            const int q = lane & 15, k = q >> 2;
-            const unsigned c = (first + ((lane >> 4) & 1) * 16 + (q & 3) * 4) * 2;
-            at[0] = (8 * h + k) * TX * 2 + (c ^ (k << 5));            // fragments 0, 2, ..
-            at[1] = (8 * h + k) * TX * 2 + ((c + 64) ^ (k << 5));     // fragments 1, 3, ..
+            for (int ks = 0; ks < KSTEPS; ks++) at[ks] = (first + l) * SLAB + (((ks * 2 + h) ^ (l >> 1 & 7)) << 4);
         } else {
+            const int q = lane & 15, k = sizeof(El) == 2 ? 8 * h + (q >> 2) : 4 * h;
 #pragma unroll
-            for (int e = 0; e < 4; e++) at[e] = (4 * h + e) * TX * 4 + ((unsigned)((first + (lane & 31)) * 4) ^ (e << 5));
+            for (int f = 0; f < 4; f++) {
+                const int byte = sizeof(El) == 2 ? (first + f * 32 + (l >> 4) * 16 + (q & 3) * 4) * 2 : (first + f * 32 + l) * 4;
+                at[f] = k * TX * (int)sizeof(El) + (turned<El, TX>(k, byte >> 4) << 4 | (byte & 15));
+            }
         }
     }
     __device__ __forceinline__ i32x4_t read(lds_bytes slab, int ks, int f) const {
@@ -199,14 +207,14 @@ struct TileReader {
             return *reinterpret_cast<vec_ptr>(slab + at[ks] + f * 32 * SLAB);
         } else if constexpr (sizeof(El) == 2) {
             typedef __attribute__((address_space(3))) s16x4_t *half_ptr;
-            const lds_bytes p = slab + at[f & 1] + (f >> 1) * 128 + ks * 16 * TX * 2;
+            const lds_bytes p = slab + at[f] + ks * 16 * TX * 2;
             const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((half_ptr)p);
             const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((half_ptr)(p + 4 * TX * 2));
             return __builtin_bit_cast(i32x4_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             i32x4_t r;
 #pragma unroll
-            for (int e = 0; e < 4; e++) r[e] = *reinterpret_cast<__attribute__((address_space(3))) int *>(slab + at[e] + f * 128 + ks * 8 * TX * 4);
+            for (int e = 0; e < 4; e++) r[e] = *reinterpret_cast<__attribute__((address_space(3))) int *>(slab + at[f] + e * TX * 4 + ks * 8 * TX * 4);
             return r;
         }
     }
@@ -364,7 +372,7 @@ struct Tile {
     }
 
     // Writes a finished tile.  The accumulators' order has four adjacent i per lane and another j in every lane.  In passes of COLS
-    // columns per row of waves, the waves put their parts side by side into LDS (f32; chunk c of column j at c ^ (j & 7): no two
+    // columns per row of waves, the waves put their parts side by side into LDS (f32; chunk c of column j at c ^ (j & 15): no two
     // lanes on one bank) and take whole columns out of it, so that a store is one run of TI outputs.  Its length matters where
     // columns do not begin on lines of 128 bytes (2,000 f32 scores a frame), because every run that a line's border cuts costs a
     // line more: 131,072 x 2,000 f32 with next to nothing to multiply take 305 us in runs of 128 bytes and 214 us in runs of 1 KB.
@@ -394,7 +402,7 @@ struct Tile {
                         const float v[4] = {(float)x[4 * b], (float)x[4 * b + 1], (float)x[4 * b + 2], (float)x[4 * b + 3]};
                         f32x4_t r;
                         pre(v, held.j[c], r);
-                        *reinterpret_cast<f32x4_t *>(st + (j - from) * ROW + (((wi * FI + f) * 8 + b * 2 + h) ^ (j & 7)) * 16) = r;
+                        *reinterpret_cast<f32x4_t *>(st + (j - from) * ROW + (((wi * FI + f) * 8 + b * 2 + h) ^ (j & 15)) * 16) = r;
                     }
             }
             if constexpr (WI > 1) lds_barrier(); else __builtin_amdgcn_wave_barrier();
@@ -404,7 +412,7 @@ struct Tile {
                 float v[V], r[V];
 #pragma unroll
                 for (int e = 0; e < V / 4; e++) {
-                    const f32x4_t x = *reinterpret_cast<const f32x4_t *>(st + col * ROW + ((lane % LPR * (V / 4) + e) ^ ((from + col) & 7)) * 16);
+                    const f32x4_t x = *reinterpret_cast<const f32x4_t *>(st + col * ROW + ((lane % LPR * (V / 4) + e) ^ ((from + col) & 15)) * 16);
 #pragma unroll
                     for (int d = 0; d < 4; d++) v[4 * e + d] = x[d];
                 }

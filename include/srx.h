@@ -458,8 +458,11 @@ int srx_em_fused_finish_dev(srx_ctx *ctx, srx_model *A, srx_model *B, const doub
  * gradients.  NO COUNTERPART IN THE REFERENCE, whose emission model is the GMM.  Buffers are row-major device memory in one
  * of three element types, row r at base + r * ld elements; sums, states, gates and scales are f32.  Every call is
  * asynchronous on the context's stream, allocates nothing and keeps nothing between calls: scratch is the caller's, so calls
- * may be captured into a graph (one scratch per graph that can run beside another).  Offset tables are DEVICE arrays and are
- * held to [0, total] by the kernels.  Output buffers overlap no other buffer unless said so. */
+ * may be captured into a graph (one scratch per graph that can run beside another).  Offset tables are DEVICE arrays of entries
+ * that do not descend; whatever they hold, kernels stay inside [0, total].  Output buffers overlap no other buffer unless said so.
+ * Addresses are multiples of the element's size (tables: 8 bytes), row strides of any size not below the row's length; 16-byte
+ * aligned rows are read and written fastest.  A call with a size, stride, address or type outside what stands here returns
+ * SRX_ERR_INVALID before anything is launched. */
 typedef enum { SRX_F32 = 0, SRX_F16 = 1, SRX_BF16 = 2 } srx_dtype;
 
 /* Gated linear recurrence along the frames of every utterance, channel by channel (beside the fixed smoothing of
@@ -473,7 +476,7 @@ typedef enum { SRX_F32 = 0, SRX_F16 = 1, SRX_BF16 = 2 } srx_dtype;
  * max_frames: the longest utterance where the caller knows it (0: unknown); it only chooses how the work is cut.
  * states_dev: srx_gated_scan_states_len floats that the backward pass reads (the state in front of every
  * SRX_SCAN_STATE_EVERY-th frame), or NULL.  scratch_dev: srx_gated_scan_scratch_bytes (which may be 0), for either pass; it
- * holds nothing between calls.  Where an utterance is cut into pieces its state passes a piece through the product of the
+ * holds nothing between calls.  At most 2^40 frames and 2^20 channels.  Where an utterance is cut into pieces its state passes a piece through the product of the
  * piece's gates: for gates beyond +-1 that product has to stay inside the f32 range. */
 enum { SRX_SCAN_VALUE = 0, SRX_SCAN_SIGMOID = 1 };
 enum { SRX_SCAN_STATE_EVERY = 16 };
@@ -500,7 +503,8 @@ int srx_gated_scan_backward_dev(srx_ctx *ctx, int mode, int dtype, const void *g
  *   srx_group_matmul_dw_dev   dW_e = sum dy_r x_r^T          -> dw [n_groups][N][K], zeros for a group of no rows;
  *                             db_e = sum dy_r                -> dbias [n_groups][N] f32, or NULL
  * in_dtype: f32, f16 or bf16 (products on the matrix cores of that type, sums in f32); out_dtype: the same or f32.  Rows of no
- * group are left as they were.  Results do not depend on the order in which the workgroups run. */
+ * group are left as they were.  Results do not depend on the order in which the workgroups run.  scratch_dev of dW: 16-byte
+ * aligned.  At most 2^40 rows, 2^20 groups, K and N of 2^20, row strides of 2^21 elements, and 2^28 tiles of the result. */
 int srx_group_matmul_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *x_dev, int64_t ld_x, const void *w_dev, const float *bias_dev,
                          const int64_t *row_off_dev, int n_groups, int64_t total_rows, int K, int N, void *y_dev, int64_t ld_y);
 int srx_group_matmul_dx_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *w_dev, const int64_t *row_off_dev,
@@ -520,7 +524,7 @@ int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const voi
  *   same call, once.
  * srx_matmul_i8_dev: y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n (the sum exact in 32 bits; bias f32 or NULL) at
  *   y[r * stride_r + n * stride_n], one of the two strides 1 (row by row: stride_n = 1; state by state: stride_r = 1), of
- *   out_dtype.  Codes may come from elsewhere: at least one operand has to hold zeros behind column K up to whole 16 bytes. */
+ *   out_dtype; code rows of at most 4 MiB, an output stride of at most 2^26.  Codes may come from elsewhere: at least one operand has to hold zeros behind column K up to whole 16 bytes. */
 enum { SRX_I8_MAX_K = 131072 };
 int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev, int64_t ld_x, int64_t rows, int K, int8_t *q_dev, int64_t ld_q, float *scale_dev);
 int srx_matmul_i8_dev(srx_ctx *ctx, int out_dtype, const int8_t *xq_dev, int64_t ld_xq, const float *xs_dev, const int8_t *wq_dev, int64_t ld_wq,

@@ -51,7 +51,7 @@ struct Magnitude {
 };
 
 // A wave takes R rows, each in NV runs of 16 bytes per lane, and reads them once; NV = 0: one row of any length, its maximum in a
-// first sweep and the codes in a second.  HBM-bound: 3 bytes per element of a 16-bit type; several short rows per wave because
+// first sweep and the codes in a second.  131,072 x 1,024 bf16: 95 us, 403 MB, 4.2 TB/s.  HBM-bound: 3 bytes per element of a 16-bit type; several short rows per wave because
 // one row's loads (2 KB at 1,024 columns) do not cover their latency.
 template <class T, int NV, int R>
 __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs p) {
@@ -140,6 +140,9 @@ struct I8Args {
 struct ScaleBias { float s, b; };
 __device__ __forceinline__ ScaleBias from_lane(const ScaleBias &v, int l) { return {__shfl(v.s, l), __shfl(v.b, l)}; }
 
+// Scales and bias on a tile's way out.  131,072 x 1,024 -> 2,000 f32: 440 to 470 us; the outputs alone (1,049 MB) are 152 us at the rate of a
+// fill, the products 255 us at the library's best rate, and within a CU one follows the other.  The sum alone runs at 2,400 TOP/s (time per
+// further K).
 template <class O, int WI, int WJ, int FI, int FJ>
 __global__ __launch_bounds__(WI *WJ * 64, 2) void k_matmul_i8(I8Args p) {
     typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, TO_LDS> T;
@@ -241,7 +244,7 @@ extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev,
 }
 
 // 32 x 32 tiles for few rows (the product is bound by reading the weights once), and where even these are no more than the chip
-// holds at a time
+// holds at a time (4 rows x 512 -> 2,000 f32: 5 us)
 static constexpr int64_t I8_THIN_ROWS = 64;
 
 template <class O, int WI, int WJ, int FI, int FJ>

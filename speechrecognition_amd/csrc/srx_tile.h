@@ -17,6 +17,12 @@
 // together, so the columns' 64-byte parts are moved by k & 3; f32 ones come element by element, both half-waves' k together, so
 // their 128-byte parts are moved by bit 2 of k (turned()).
 //
+// Bound by the matrix cores and what stands beside them: a workgroup of 256 x 256 fills a CU's LDS and half its registers, so its first
+// loads and its stores run beside nobody's products (8 groups, 65,536 rows, 1,024 x 1,024 bf16: matrix cores busy 0.49 of the time,
+// forward 170 us or 810 TFLOP/s; 16,384 x 4,096 x 4,096: 1,087).  Tried and slower: slabs of 64 bytes four or five deep (10 %),
+// touching the slab after next for the L2 (15 %), four waves of 128 x 128, workgroups that stay and take tile after tile (loads
+// wait behind the stores of the tile before them: the counter of memory operations is in order).
+//
 // Result layout: lane l holds column j = l & 31, rows 8 b + 4 (l >> 5) + 0..3 for b = 0..3: four adjacent i for one j.
 #pragma once
 #include <type_traits>

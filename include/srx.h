@@ -476,7 +476,8 @@ typedef enum { SRX_F32 = 0, SRX_F16 = 1, SRX_BF16 = 2 } srx_dtype;
  * max_frames: the longest utterance where the caller knows it (0: unknown); it only chooses how the work is cut.
  * states_dev: srx_gated_scan_states_len floats that the backward pass reads (the state in front of every
  * SRX_SCAN_STATE_EVERY-th frame), or NULL.  scratch_dev: srx_gated_scan_scratch_bytes (which may be 0), for either pass; it
- * holds nothing between calls.  At most 2^40 frames and 2^20 channels.  Where an utterance is cut into pieces its state passes a piece through the product of the
+ * holds nothing between calls.  At most 2^40 frames, 2^20 channels, and 2^25 utterances times 64 channels (2^22 utterances where
+ * they are cut).  Where an utterance is cut into pieces its state passes a piece through the product of the
  * piece's gates: for gates beyond +-1 that product has to stay inside the f32 range. */
 enum { SRX_SCAN_VALUE = 0, SRX_SCAN_SIGMOID = 1 };
 enum { SRX_SCAN_STATE_EVERY = 16 };
@@ -504,7 +505,8 @@ int srx_gated_scan_backward_dev(srx_ctx *ctx, int mode, int dtype, const void *g
  *                             db_e = sum dy_r                -> dbias [n_groups][N] f32, or NULL
  * in_dtype: f32, f16 or bf16 (products on the matrix cores of that type, sums in f32); out_dtype: the same or f32.  Rows of no
  * group are left as they were.  Results do not depend on the order in which the workgroups run.  scratch_dev of dW: 16-byte
- * aligned.  At most 2^40 rows, 2^20 groups, K and N of 2^20, row strides of 2^21 elements, and 2^28 tiles of the result. */
+ * aligned.  At most 2^40 rows, 2^20 groups, K and N of 2^20, row strides of 2^21 elements, and 2^22 tiles of the result (of 32 x 32
+ * up to 256 x 256 elements, never fewer than the groups). */
 int srx_group_matmul_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *x_dev, int64_t ld_x, const void *w_dev, const float *bias_dev,
                          const int64_t *row_off_dev, int n_groups, int64_t total_rows, int K, int N, void *y_dev, int64_t ld_y);
 int srx_group_matmul_dx_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *w_dev, const int64_t *row_off_dev,
@@ -516,7 +518,7 @@ int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const voi
 
 /* 8-bit matrix product with a scale for each row and each output (beside srx_gmm_score_dev: emission scores of an output layer
  * over the tied states, in the strides that srx_viterbi_* reads).
- * srx_quantize_rows_dev: scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded to the nearest whole
+ * srx_quantize_rows_dev (less than 2^26 rows): scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded to the nearest whole
  *   number, ties to even; a row of zeros has scale 0 and codes 0 (and where the
  *   scale lies below the normal range, codes are held to +-127); a row that holds a NaN or an infinity has that as its scale
  *   and codes 0, so that its outputs are NaN.  x: [rows][ld >= K] of `dtype`; codes: [rows][ld_q], ld_q a multiple of 16 bytes,

@@ -34,3 +34,6 @@ __device__ __forceinline__ typename SrxVec<T, V>::type srx_pack(const float (&f)
 }
 
 static inline bool srx_aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+// A launch takes less than 2^32 threads along a dimension
+static inline bool srx_grid_fits(int64_t blocks, int threads) { return blocks < (1ll << 32) / threads; }

@@ -387,7 +387,7 @@ static int group_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
     typedef Tile<El, WI, WJ, FI, FJ, DX, false, HOW> T;
     p.tiles_i = ceil_div64(DX ? p.K : p.N, T::TI);
     p.tiles_j = p.total / T::TJ + p.E;
-    SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
+    SRX_REQUIRE(ctx, srx_grid_fits(p.tiles_i * p.tiles_j, T::NT), "%s: too many tiles", name);
     SrxProf prof_(ctx, DX ? "k_group_dx" : "k_group");
     hipLaunchKernelGGL((k_group<El, O, DX, WI, WJ, FI, FJ, HOW>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
     return SRX_OK;
@@ -396,7 +396,7 @@ static int group_tile(srx_ctx *ctx, const char *name, GroupArgs &p) {
 template <class El, class O, bool DX, int NKS>
 static int group_small(srx_ctx *ctx, const char *name, GroupArgs &p) {
     const int64_t blocks = ceil_div64(p.total / SMALL_ROWS + p.E, 4);
-    SRX_REQUIRE(ctx, blocks < (1ll << 28), "%s: too many tiles", name);
+    SRX_REQUIRE(ctx, srx_grid_fits(blocks, 256), "%s: too many tiles", name);
     SrxProf prof_(ctx, DX ? "k_group_dx" : "k_group");
     hipLaunchKernelGGL((k_group_small<El, O, DX, NKS>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
     return SRX_OK;
@@ -410,7 +410,7 @@ static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
         if (p.K < 16 / Z || group_thin(ctx, p.total, p.E, p.N)) {
             p.tiles_i = ceil_div64(p.N, 32);
             p.tiles_j = p.total / 32 + p.E;
-            SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
+            SRX_REQUIRE(ctx, srx_grid_fits(p.tiles_i * p.tiles_j, THIN_WAVES * 64), "%s: too many tiles", name);
             SrxProf prof_(ctx, "k_group_thin");
             hipLaunchKernelGGL((k_group_thin<El, O>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(THIN_WAVES * 64), 0, ctx->stream, p);
             return SRX_OK;

@@ -202,7 +202,7 @@ __global__ __launch_bounds__(THIN_WAVES * 64) void k_matmul_i8_thin(I8Args p) {
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-static constexpr int64_t I8_MAX_ROWS = 1ll << 40;
+static constexpr int64_t I8_MAX_ROWS = 1ll << 40, QUANT_MAX_ROWS = 1ll << 26;
 
 // Several rows to a wave from this many rows on: fewer are better spread over the chip, one to a wave
 static constexpr int64_t QUANT_MANY = 16384;
@@ -226,7 +226,8 @@ extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev,
     const char *name = "srx_quantize_rows_dev";
     SRX_ENTER(ctx, name);
     SRX_REQUIRE(ctx, srx_dtype_size(dtype) != 0, "%s: element type %d", name, dtype);
-    SRX_REQUIRE(ctx, rows >= 0 && rows < (1ll << 33) && K >= 1 && K <= SRX_I8_MAX_K, "%s: %lld rows of %d (at most %d)", name, (long long)rows, K, SRX_I8_MAX_K);
+    SRX_REQUIRE(ctx, rows >= 0 && rows < QUANT_MAX_ROWS && K >= 1 && K <= SRX_I8_MAX_K, "%s: %lld rows of %d (less than %lld of at most %d)", name, (long long)rows, K, (long long)QUANT_MAX_ROWS,
+                SRX_I8_MAX_K);
     if (rows == 0) return SRX_OK;
     SRX_REQUIRE(ctx, x_dev && q_dev && scale_dev, "%s: null argument", name);
     SRX_REQUIRE(ctx, ld_x >= K && ld_q >= (K + 15) / 16 * 16 && ld_q % 16 == 0 && srx_aligned(q_dev, 16),
@@ -252,7 +253,7 @@ static int i8_tile(srx_ctx *ctx, const char *name, I8Args &p) {
     typedef Tile<int8_t, WI, WJ, FI, FJ, false, false, TO_LDS> T;
     p.tiles_i = ceil_div64(p.I, T::TI);
     p.tiles_j = ceil_div64(p.J, T::TJ);
-    SRX_REQUIRE(ctx, p.tiles_i * p.tiles_j < (1ll << 28), "%s: too many tiles", name);
+    SRX_REQUIRE(ctx, srx_grid_fits(p.tiles_i * p.tiles_j, T::NT), "%s: too many tiles", name);
     SrxProf prof_(ctx, "k_matmul_i8");
     hipLaunchKernelGGL((k_matmul_i8<O, WI, WJ, FI, FJ>), dim3((unsigned)(p.tiles_i * p.tiles_j)), dim3(T::NT), 0, ctx->stream, p);
     return SRX_OK;

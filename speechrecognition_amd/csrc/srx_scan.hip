@@ -491,7 +491,7 @@ static int scan_run(srx_ctx *ctx, const char *name, int mode, int dtype, ScanArg
         p.B = p.A + pl.pieces * p.D;
     }
     const int64_t waves = (pl.L ? pl.pieces : p.n_utt) * ceil_div64(p.D, 64);
-    SRX_REQUIRE(ctx, waves < (1ll << 31), "%s: too many utterances and channels", name);
+    SRX_REQUIRE(ctx, srx_grid_fits(ceil_div64(waves, 4), 256) && (!pl.L || srx_grid_fits(p.n_utt, 64 * CW)), "%s: too many utterances and channels", name);
     // `lines`: every row starts on a 128-byte line
     bool wide = p.D % 2 == 0, lines = true;
     const size_t z = srx_dtype_size(dtype);

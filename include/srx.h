@@ -518,15 +518,17 @@ int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const voi
 
 /* 8-bit matrix product with a scale for each row and each output (beside srx_gmm_score_dev: emission scores of an output layer
  * over the tied states, in the strides that srx_viterbi_* reads).
- * srx_quantize_rows_dev (less than 2^26 rows): scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded to the nearest whole
- *   number, ties to even; a row of zeros has scale 0 and codes 0 (and where the
- *   scale lies below the normal range, codes are held to +-127); a row that holds a NaN or an infinity has that as its scale
- *   and codes 0, so that its outputs are NaN.  x: [rows][ld >= K] of `dtype`; codes: [rows][ld_q], ld_q a multiple of 16 bytes,
+ * srx_quantize_rows_dev (less than 2^26 rows): scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded
+ *   to the nearest whole number, ties to even; a row of zeros has scale 0 and codes 0 (and where the scale lies below the normal
+ *   range, codes are held to +-127); a row that holds a NaN or an infinity has that as its scale and codes 0, so that its outputs
+ *   are NaN.  x: [rows][ld >= K] of `dtype`; codes: [rows][ld_q], ld_q a multiple of 16 bytes,
  *   q_dev 16-byte aligned, zeros written behind column K up to whole 16 bytes.  Weights (rows = outputs) are quantised by the
  *   same call, once.
- * srx_matmul_i8_dev: y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n (the sum exact in 32 bits; bias f32 or NULL) at
+ * srx_matmul_i8_dev: y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n (the sum exact in 32 bits, its products with either scale
+ *   inside the f32 range; bias f32 or NULL) at
  *   y[r * stride_r + n * stride_n], one of the two strides 1 (row by row: stride_n = 1; state by state: stride_r = 1), of
- *   out_dtype; code rows of at most 4 MiB, an output stride of at most 2^26.  Codes may come from elsewhere: at least one operand has to hold zeros behind column K up to whole 16 bytes. */
+ *   out_dtype; code rows of at most 4 MiB, an output stride of at most 2^26.  Codes may come from elsewhere: at least one
+ *   operand has to hold zeros behind column K up to whole 16 bytes. */
 enum { SRX_I8_MAX_K = 131072 };
 int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev, int64_t ld_x, int64_t rows, int K, int8_t *q_dev, int64_t ld_q, float *scale_dev);
 int srx_matmul_i8_dev(srx_ctx *ctx, int out_dtype, const int8_t *xq_dev, int64_t ld_xq, const float *xs_dev, const int8_t *wq_dev, int64_t ld_wq,

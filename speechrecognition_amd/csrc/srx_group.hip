@@ -428,8 +428,11 @@ static int group_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
     // W is read along its columns (extent K) by dx, along its rows (K) by the forward product
     const bool dma = tile_dma(p.w, p.K, p.K, Z) && (DX ? tile_dma(p.dy, p.ld_dy, p.N, Z) : tile_dma(p.x, p.ld_x, p.K, Z));
     if (!dma) return group_tile<El, O, DX, 2, 2, 2, 2, BY_RUN>(ctx, name, p);
-    if (tile_large(ceil_div64(I, 256) * (p.total / 256 + (p.E + 1) / 2), ceil_div64(I, 128) * (p.total / 128 + (p.E + 1) / 2), ctx->num_cus))
-        return group_tile<El, O, DX, 4, 2, 2, 4, TO_LDS>(ctx, name, p);
+    // f32 products take the matrix cores eight times as long for the same bytes, so that nothing is gained by reading operands less often,
+    // and two workgroups to a CU hide each other's first loads and stores: 32,768 rows of 1,024 -> 1,024 558 us, 723 in 256 x 256 tiles
+    if constexpr (Z == 2)
+        if (tile_large(ceil_div64(I, 256) * (p.total / 256 + (p.E + 1) / 2), ceil_div64(I, 128) * (p.total / 128 + (p.E + 1) / 2), ctx->num_cus))
+            return group_tile<El, O, DX, 4, 2, 2, 4, TO_LDS>(ctx, name, p);
     return group_tile<El, O, DX, 2, 2, 2, 2, TO_LDS>(ctx, name, p);
 }
 
@@ -522,7 +525,9 @@ static int group_dw_launch(srx_ctx *ctx, const char *name, GroupArgs &p) {
     constexpr int Z = sizeof(El);
     if (p.N < 16 / Z || p.K < 16 / Z) return group_dw_tile<El, O, 2, 2, 2, 2, BY_ELEMENT>(ctx, name, p);
     if (!tile_dma(p.x, p.ld_x, p.K, Z) || !tile_dma(p.dy, p.ld_dy, p.N, Z)) return group_dw_tile<El, O, 2, 2, 2, 2, BY_RUN>(ctx, name, p);
-    return dw_large(ctx, p.E, p.total, p.K, p.N) ? group_dw_tile<El, O, 4, 2, 2, 4, TO_LDS>(ctx, name, p) : group_dw_tile<El, O, 2, 2, 2, 2, TO_LDS>(ctx, name, p);
+    if constexpr (Z == 2)   // (f32: within 2 % of each other)
+        if (dw_large(ctx, p.E, p.total, p.K, p.N)) return group_dw_tile<El, O, 4, 2, 2, 4, TO_LDS>(ctx, name, p);
+    return group_dw_tile<El, O, 2, 2, 2, 2, TO_LDS>(ctx, name, p);
 }
 
 extern "C" int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const void *dy_dev, int64_t ld_dy, const void *x_dev, int64_t ld_x,

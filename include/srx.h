@@ -39,12 +39,15 @@ typedef enum {
 typedef struct srx_ctx srx_ctx;
 
 /* ---------------------------------------------------------------- context ---------- */
-/* One per GPU.  `stream` is a hipStream_t to launch on (NULL: the context creates its own). */
+/* One per GPU.  `stream` is a hipStream_t to launch on (NULL: the context creates its own, which waits for no other stream and
+ * which no other stream waits for).  SRX_STREAM_DEFAULT: the device's default stream, whose handle is NULL -- the one that torch works
+ * on unless told otherwise; calls are then ordered with that work, and nothing else is needed. */
+#define SRX_STREAM_DEFAULT ((void *)1)
 int srx_ctx_create(int device, void *stream, srx_ctx **out);
 void srx_ctx_destroy(srx_ctx *ctx);
 const char *srx_last_error(const srx_ctx *ctx); /* ctx may be NULL: last creation error */
 int srx_sync(srx_ctx *ctx);
-/* The hipStream_t the context launches on (the one given to srx_ctx_create, or its own).  No counterpart in the reference
+/* The hipStream_t the context launches on (the one given to srx_ctx_create, or its own; NULL is the device's default stream).  No counterpart in the reference
  * (which has no streams): lets a caller order its own work -- copies, RCCL collectives, torch ops -- against libsrx's
  * kernels on the device instead of calling srx_sync. */
 void *srx_ctx_stream(const srx_ctx *ctx);

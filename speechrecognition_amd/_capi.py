@@ -19,6 +19,7 @@ SRX_SCORE_MFMA = 0
 SRX_SCORE_EXACT = 1
 SRX_SCORE_MFMA_F16X3 = 2
 SRX_COMM_ID_BYTES = 128
+SRX_STREAM_DEFAULT = 1
 SRX_F32 = 0
 SRX_F16 = 1
 SRX_BF16 = 2

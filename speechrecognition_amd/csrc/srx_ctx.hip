@@ -25,7 +25,9 @@ extern "C" int srx_ctx_create(int device, void *stream, srx_ctx **out) {
     srx_ctx *c = new srx_ctx();
     c->device = device;
     c->num_cus = prop.multiProcessorCount;
-    if (stream) {
+    if (stream == SRX_STREAM_DEFAULT) {
+        c->stream = nullptr;
+    } else if (stream) {
         c->stream = reinterpret_cast<hipStream_t>(stream);
     } else {
         hipError_t es = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);

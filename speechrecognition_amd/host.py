@@ -22,12 +22,15 @@ def _ptr(a):
 
 
 class Context:
-    """srx_ctx: one per GPU.  `stream` is a raw hipStream_t handle (int) or None."""
+    """srx_ctx: one per GPU.  `stream` is a raw hipStream_t handle (int), 0 being the device's default stream, or None: a stream of
+    the context's own.  torch.cuda.current_stream().cuda_stream puts the calls in order with torch's work on that stream; against a
+    stream of its own the caller orders them (stream_handle())."""
 
     def __init__(self, device=0, stream=None):
         self.lib = _capi.load()
         h = C.c_void_p()
-        check(self.lib.srx_ctx_create(device, C.c_void_p(stream) if stream else None, C.byref(h)))
+        given = None if stream is None else C.c_void_p(stream or _capi.SRX_STREAM_DEFAULT)
+        check(self.lib.srx_ctx_create(device, given, C.byref(h)))
         self.h = h
         self.device = device
 

@@ -162,19 +162,21 @@ _kept = {}
 
 
 def _context():
-    """The context that a program keeps, on the device of the moment."""
-    if "ctx" not in _kept:
+    """What a program keeps for torch's current stream and its device: a context on that stream, so that the calls stand in order with
+    what made their inputs and with what reads their outputs, and the scratch memory of its calls."""
+    stream = torch.accelerator.current_stream()  # (the look-up that costs least)
+    kept = _kept.get(stream)
+    if kept is None:
         from speechrecognition_amd import host
-        _kept["host"], _kept["ctx"] = host, host.Context(torch.cuda.current_device())
-    return _kept["host"], _kept["ctx"]
+        kept = _kept[stream] = (host, host.Context(stream.device_index, torch.cuda.current_stream().cuda_stream), {})
+    return kept
 
 
-def _scratch(name, nbytes):
+def _scratch(room, name, nbytes):
     """Scratch memory that a program keeps from call to call, as large as the largest call so far needs."""
-    b = _kept.get(name)
+    b = room.get(name)
     if b is None or b.numel() < nbytes:
-        torch.cuda.synchronize()
-        b = _kept[name] = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device="cuda")
+        b = room[name] = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device="cuda")
     return b
 
 
@@ -195,11 +197,11 @@ def _doubling(a, h, longest):
 
 def _scan(s):
     if own:
-        host, ctx = _context()
+        host, ctx, room = _context()
         n, total, dim, longest = s["n"], s["x"].shape[0], s["dim"], s["longest"]
         mode = host.SCAN_SIGMOID if s["kind"] == "sigmoid" else host.SCAN_VALUE
-        scratch = _scratch("scan", host.gated_scan_scratch_bytes(ctx, n, total, longest, dim))
-        states = _scratch("states", host.gated_scan_states_bytes(ctx, n, total, dim)) if s["train"] else None
+        scratch = _scratch(room, "scan", host.gated_scan_scratch_bytes(ctx, n, total, longest, dim))
+        states = _scratch(room, "states", host.gated_scan_states_bytes(ctx, n, total, dim)) if s["train"] else None
         host.gated_scan(ctx, mode, s["gate"], s["x"], s["off"], longest, s["h"], h0=s["h0"], h_last=s["h_last"], states=states,
                         scratch=scratch)
         if not s["train"]:
@@ -249,12 +251,12 @@ def _padded(x, s):
 
 def _group(s):
     if own:
-        host, ctx = _context()
+        host, ctx, room = _context()
         host.group_matmul(ctx, s["x"], s["w"], s["off"], s["y"], bias=s["bias"])
         if not s["train"]:
             return {"y": s["y"]}
         host.group_matmul_dx(ctx, s["dy"], s["w"], s["off"], s["dx"])
-        scratch = _scratch("group", host.group_matmul_dw_scratch_bytes(ctx, s["n"], s["x"].shape[0], s["k"], s["m"]))
+        scratch = _scratch(room, "group", host.group_matmul_dw_scratch_bytes(ctx, s["n"], s["x"].shape[0], s["k"], s["m"]))
         host.group_matmul_dw(ctx, s["dy"], s["x"], s["off"], s["dw"], dbias=s["dbias"], scratch=scratch)
         return {k: s[k] for k in ("y", "dx", "dw", "dbias")}
     o = s["y"].dtype
@@ -272,7 +274,7 @@ def _group(s):
 
 def _i8(s):
     if own:
-        host, ctx = _context()
+        host, ctx, _ = _context()
         host.quantize_rows(ctx, s["x"], s["xq"], s["xs"])
         host.matmul_i8(ctx, s["xq"], s["xs"], s["wq"], s["ws"], s["k"], s["y"], bias=s["bias"])
         return {"y": s["y"]}

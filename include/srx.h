@@ -527,8 +527,8 @@ int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const voi
  *   are NaN.  x: [rows][ld >= K] of `dtype`; codes: [rows][ld_q], ld_q a multiple of 16 bytes,
  *   q_dev 16-byte aligned, zeros written behind column K up to whole 16 bytes.  Weights (rows = outputs) are quantised by the
  *   same call, once.
- * srx_matmul_i8_dev: y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n (the sum exact in 32 bits, its products with either scale
- *   inside the f32 range; bias f32 or NULL) at
+ * srx_matmul_i8_dev: y(r, n) = xs_r ws_n sum_k xq_rk wq_nk + bias_n (the sum exact for all codes from -128 to 127, its products with
+ *   either scale inside the f32 range; bias f32 or NULL) at
  *   y[r * stride_r + n * stride_n], one of the two strides 1 (row by row: stride_n = 1; state by state: stride_r = 1), of
  *   out_dtype; code rows of at most 4 MiB, an output stride of at most 2^26.  Codes may come from elsewhere: at least one
  *   operand has to hold zeros behind column K up to whole 16 bytes. */

@@ -3,7 +3,7 @@
 //   s_r = max_k |x_rk| / 127,  q_rk = round(x_rk / s_r) to the nearest whole number, ties to even   (s_r = 0: all codes 0)
 //   y_rn = s_r s_n sum_k q_rk q_nk + b_n
 //
-// The sum is exact in 32 bits (K <= SRX_I8_MAX_K), so the only roundings are the scale's, the codes' and the output's few.
+// The sum is exact in 32 bits (K <= SRX_I8_MAX_K, see full_sum), so the only roundings are the scale's, the codes' and the output's few.
 #include "srx_tile.h"
 
 struct QuantArgs {
@@ -137,6 +137,15 @@ struct I8Args {
     int64_t tiles_i, tiles_j;
 };
 
+// Sums lie in (-2^31, 2^31], since a product of two codes lies in [-127 * 128, 128 * 128] and there are at most 2^17 of them.  The one
+// that 32 bits do not hold, 2^31, needs all of the 2^17 products at their largest, and comes out as -2^31, which no other sum is.
+static_assert(SRX_I8_MAX_K == 1 << 17, "full_sum");
+__device__ __forceinline__ void full_sum(int K, float (&v)[4]) {
+    if (K < SRX_I8_MAX_K) return;   // (the same for all lanes)
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = v[e] == -0x1p31f ? 0x1p31f : v[e];
+}
+
 struct ScaleBias { float s, b; };
 __device__ __forceinline__ ScaleBias from_lane(const ScaleBias &v, int l) { return {__shfl(v.s, l), __shfl(v.b, l)}; }
 
@@ -167,7 +176,12 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_matmul_i8(I8Args p) {
     float none[FJ];
     T::template product<false>(smem, P, Q, (p.K + 15) / 16 * 16, acc, none, false);
     T::template write_out<O>(
-        smem, acc, held, [](const float (&v)[4], const ScaleBias &j, f32x4_t &r) { r = {v[0] * j.s, v[1] * j.s, v[2] * j.s, v[3] * j.s}; },
+        smem, acc, held,
+        [&](const float (&sum)[4], const ScaleBias &j, f32x4_t &r) {
+            float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+            full_sum(p.K, v);
+            r = {v[0] * j.s, v[1] * j.s, v[2] * j.s, v[3] * j.s};
+        },
         [&](const float (&v)[RUN<O>], const ScaleBias (&i)[RUN<O>], auto &&j, float (&r)[RUN<O>]) {
 #pragma unroll
             for (int e = 0; e < RUN<O>; e++) r[e] = __builtin_fmaf(v[e], i[e].s, i[e].b);
@@ -188,8 +202,10 @@ __global__ __launch_bounds__(THIN_WAVES * 64) void k_matmul_i8_thin(I8Args p) {
     const TileOperand P{p.p + i0 * p.ld_p, p.ld_p, (int)(p.I - i0 < 32 ? p.I - i0 : 32), 0};
     const TileOperand Q{p.q + j0 * p.ld_q, p.ld_q, (int)(p.J - j0 < 32 ? p.J - j0 : 32), 0};
     O *y = reinterpret_cast<O *>(p.y);
-    thin_product<int8_t>(smem, P, Q, (p.K + 15) / 16 * 16, [&](int i, int j, const float (&v)[4]) {
+    thin_product<int8_t>(smem, P, Q, (p.K + 15) / 16 * 16, [&](int i, int j, const float (&sum)[4]) {
         if (j >= Q.n || i >= P.n) return;
+        float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+        full_sum(p.K, v);
         const float sj = p.sq[j0 + j], bj = p.bias && !p.bias_i ? p.bias[j0 + j] : 0.0f;
         float f[4];
 #pragma unroll

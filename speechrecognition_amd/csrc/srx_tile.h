@@ -529,10 +529,17 @@ __device__ __forceinline__ void thin_product(unsigned char *smem, const TileOper
     __syncthreads();
     if (t < 256) {
         const int oj = t >> 3, c = t & 7;
-        val4 v = st[oj * 8 + (c ^ (oj & 7))];
+        typedef std::conditional_t<std::is_same<val, int>::value, unsigned, val> part;   // (whole numbers: a sum past the range wraps)
+        part v[4];
 #pragma unroll
-        for (int w = 1; w < THIN_WAVES; w++) v += st[(w * 32 + oj) * 8 + (c ^ (oj & 7))];
-        const float f[4] = {(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+        for (int e = 0; e < 4; e++) v[e] = (part)st[oj * 8 + (c ^ (oj & 7))][e];
+#pragma unroll
+        for (int w = 1; w < THIN_WAVES; w++) {
+            const val4 more = st[(w * 32 + oj) * 8 + (c ^ (oj & 7))];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += (part)more[e];
+        }
+        const float f[4] = {(float)(val)v[0], (float)(val)v[1], (float)(val)v[2], (float)(val)v[3]};
         emit(c * 4, oj, f);
     }
 }

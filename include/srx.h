@@ -521,7 +521,7 @@ int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const voi
 
 /* 8-bit matrix product with a scale for each row and each output (beside srx_gmm_score_dev: emission scores of an output layer
  * over the tied states, in the strides that srx_viterbi_* reads).
- * srx_quantize_rows_dev (less than 2^26 rows): scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded
+ * srx_quantize_rows_dev (less than 2^26 rows; of more than 4 KiB each: at most 2^26 - 4): scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded
  *   to the nearest whole number, ties to even; a row of zeros has scale 0 and codes 0 (and where the scale lies below the normal
  *   range, codes are held to +-127); a row that holds a NaN or an infinity has that as its scale and codes 0, so that its outputs
  *   are NaN.  x: [rows][ld >= K] of `dtype`; codes: [rows][ld_q], ld_q a multiple of 16 bytes,

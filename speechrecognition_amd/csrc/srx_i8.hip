@@ -224,18 +224,22 @@ static constexpr int64_t I8_MAX_ROWS = 1ll << 40, QUANT_MAX_ROWS = 1ll << 26;
 static constexpr int64_t QUANT_MANY = 16384;
 
 template <class T, int NV, int R>
-static void quant_rows(srx_ctx *ctx, const QuantArgs &p) {
-    hipLaunchKernelGGL((k_quantize_rows<T, NV, R>), dim3((unsigned)ceil_div64(p.rows, 4 * R)), dim3(256), 0, ctx->stream, p);
+static int quant_rows(srx_ctx *ctx, const char *name, const QuantArgs &p) {
+    const int64_t blocks = ceil_div64(p.rows, 4 * R);
+    SRX_REQUIRE(ctx, srx_grid_fits(blocks, 256), "%s: %lld rows of %d: no launch holds one wave to each", name, (long long)p.rows, p.K);
+    SrxProf prof_(ctx, "k_quantize_rows");
+    hipLaunchKernelGGL((k_quantize_rows<T, NV, R>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
+    return SRX_OK;
 }
 template <class T>
-static void quant_launch(srx_ctx *ctx, const QuantArgs &p) {
+static int quant_launch(srx_ctx *ctx, const char *name, const QuantArgs &p) {
     const int runs = (int)ceil_div64(p.K, 64 * RUN<T>);
     const bool many = p.rows >= QUANT_MANY;
-    if (runs == 1) { if (many) quant_rows<T, 1, 8>(ctx, p); else quant_rows<T, 1, 1>(ctx, p); }
-    else if (runs == 2) { if (many) quant_rows<T, 2, 4>(ctx, p); else quant_rows<T, 2, 1>(ctx, p); }
-    else if (runs <= 4) { if (many) quant_rows<T, 4, 2>(ctx, p); else quant_rows<T, 4, 1>(ctx, p); }
-    else if (runs <= 8) quant_rows<T, 8, 1>(ctx, p);
-    else quant_rows<T, 0, 1>(ctx, p);
+    if (runs == 1) return many ? quant_rows<T, 1, 8>(ctx, name, p) : quant_rows<T, 1, 1>(ctx, name, p);
+    if (runs == 2) return many ? quant_rows<T, 2, 4>(ctx, name, p) : quant_rows<T, 2, 1>(ctx, name, p);
+    if (runs <= 4) return many ? quant_rows<T, 4, 2>(ctx, name, p) : quant_rows<T, 4, 1>(ctx, name, p);
+    if (runs <= 8) return quant_rows<T, 8, 1>(ctx, name, p);
+    return quant_rows<T, 0, 1>(ctx, name, p);
 }
 
 extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev, int64_t ld_x, int64_t rows, int K, int8_t *q_dev, int64_t ld_q, float *scale_dev) {
@@ -250,12 +254,8 @@ extern "C" int srx_quantize_rows_dev(srx_ctx *ctx, int dtype, const void *x_dev,
                 "%s: row strides %lld / %lld for %d columns (codes: whole 16 bytes, 16-byte aligned)", name, (long long)ld_x, (long long)ld_q, K);
     SRX_REQUIRE(ctx, srx_aligned(x_dev, srx_dtype_size(dtype)) && srx_aligned(scale_dev, 4), "%s: misaligned buffer", name);
     const QuantArgs p{x_dev, ld_x, rows, ld_q, K, q_dev, scale_dev};
-    {
-        SrxProf prof_(ctx, "k_quantize_rows");
-        if (dtype == SRX_F32) quant_launch<float>(ctx, p);
-        else if (dtype == SRX_F16) quant_launch<srx_f16>(ctx, p);
-        else quant_launch<srx_bf16>(ctx, p);
-    }
+    const int rc = dtype == SRX_F32 ? quant_launch<float>(ctx, name, p) : dtype == SRX_F16 ? quant_launch<srx_f16>(ctx, name, p) : quant_launch<srx_bf16>(ctx, name, p);
+    if (rc != SRX_OK) return rc;
     SRX_LAUNCH_CHECK(ctx);
     return SRX_OK;
 }

@@ -31,3 +31,28 @@ def test_largest_sums_of_any_codes(ctx, rows, N, by_state, out):
     assert float(want.max()) == 2.0 ** 31
     assert torch.equal((y.t() if by_state else y).double(), want)
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,z", [(_capi.SRX_F32, 4), (_capi.SRX_F16, 2), (_capi.SRX_BF16, 2)])
+def test_more_rows_than_a_launch_takes_are_refused(ctx, dtype, z):
+    """A wave to a row, four to a workgroup: refused before anything is read, the addresses are those of a small buffer."""
+    import torch
+    p = torch.zeros(4096, device="cuda").data_ptr()
+    for K in (4096 // z + 1, 8192 // z, 8192 // z + 1):
+        for rows in ((1 << 26) - 3, (1 << 26) - 1, 1 << 26):
+            assert ctx.lib.srx_quantize_rows_dev(ctx.h, dtype, p, 1 << 20, rows, K, p, 1 << 20, p) == _capi.SRX_ERR_INVALID, (rows, K)
+    ctx.sync()
+
+
+def test_most_rows_that_a_launch_takes(ctx):
+    """2^26 - 1 rows of one element: the codes are signs times 127."""
+    import torch
+    rows = (1 << 26) - 1
+    x = torch.empty((rows, 1), device="cuda").normal_()
+    q, s = torch.full((rows, 16), 7, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    torch.cuda.synchronize()
+    host.quantize_rows(ctx, x, q, s)
+    ctx.sync()
+    assert torch.equal(q[:, 0].float(), 127 * torch.sign(x[:, 0])) and not q[:, 1:].any() and torch.equal(s, x[:, 0].abs() / torch.full((1,), 127.0, device="cuda"))
+    del x, q, s
+    torch.cuda.empty_cache()

@@ -481,7 +481,8 @@ typedef enum { SRX_F32 = 0, SRX_F16 = 1, SRX_BF16 = 2 } srx_dtype;
  * SRX_SCAN_STATE_EVERY-th frame), or NULL.  scratch_dev: srx_gated_scan_scratch_bytes (which may be 0), for either pass; it
  * holds nothing between calls.  At most 2^40 frames, 2^20 channels, and 2^25 utterances times 64 channels (2^22 utterances where
  * they are cut).  Where an utterance is cut into pieces its state passes a piece through the product of the
- * piece's gates: for gates beyond +-1 that product has to stay inside the f32 range. */
+ * piece's gates: for gates beyond +-1 that product has to stay inside the f32 range.  Infinities pass a piece as they pass its
+ * frames one by one. */
 enum { SRX_SCAN_VALUE = 0, SRX_SCAN_SIGMOID = 1 };
 enum { SRX_SCAN_STATE_EVERY = 16 };
 int64_t srx_gated_scan_scratch_bytes(const srx_ctx *ctx, int n_utt, int64_t total_frames, int64_t max_frames, int D); /* -1: bad size */

@@ -11,8 +11,8 @@
 // state and gradient are f32 throughout, every output is rounded once.
 //
 // Measured (a large copy moves 5.0 TB/s): 499,674 frames x 512 bf16 in 1,000 utterances, SIGMOID: forward 370 us, 1,600 MB with the
-// states, 4.3 TB/s; backward 615 us, 2,630 MB, 4.3 TB/s.  One recording of 120,000 x 1,024 f16, VALUE, cut: forward 80 + 17 + 145 us,
-// backward 79 + 16 + 238.  1,000 x 39 f32 channels, cut: 31 + 9 + 43 us; 25 of a wave's 64 lanes idle and rows of 156 bytes.
+// states, 4.3 TB/s; backward 615 us, 2,630 MB, 4.3 TB/s.  One recording of 120,000 x 1,024 f16, VALUE, cut: forward 80 + 18 + 145 us,
+// backward 79 + 18 + 238.  1,000 x 39 f32 channels, cut: 30 + 10 + 43 us; 25 of a wave's 64 lanes idle and rows of 156 bytes.
 //
 // A segment is a whole utterance where the utterances are many and alike; otherwise every utterance is cut into pieces of L
 // frames: (1) k_scan_agg reduces each piece to (A, B) with state_out = A state_in + B, (2) k_scan_carry runs the pieces of an
@@ -308,10 +308,25 @@ __global__ __launch_bounds__(256) void k_scan_back(ScanArgs p) {
 }
 
 // Products of gates.  Gates above 1 (VALUE only) can overflow a piece's product: a gate of exactly zero still ends it, and a
-// state of exactly zero still stays zero through it.
+// state of exactly zero still stays zero through it.  Gates below 1 let it underflow: it is then left at +-GONE, which a finite
+// state does not pass and an infinite one does, with its sign, as it passes the gates one by one; exactly zero is a product
+// that holds a gate of zero (and no infinity passes: NaN).
+static constexpr float GONE = 0x1p-149f;
 template <int MODE>
-__device__ __forceinline__ float chain(float A, float a) { return MODE == SRX_SCAN_VALUE && a == 0.0f ? 0.0f : A * a; }
-__device__ __forceinline__ float carry(float A, float B, float s) { return s == 0.0f ? B : __builtin_fmaf(A, s, B); }
+struct Gates {
+    float product = 1.0f, least = 1.0f;
+    __device__ __forceinline__ void take(float a) {
+        product *= a;
+        if (MODE == SRX_SCAN_VALUE) least = __builtin_elementwise_minimum(least, fabsf(a));   // (a sigmoid is never zero)
+    }
+    __device__ __forceinline__ float all() const { return least == 0.0f ? 0.0f : fabsf(product) < GONE ? __builtin_copysignf(GONE, product) : product; }
+};
+// A s + B; one comparison on the way of s, since this is what a walk over pieces waits for
+__device__ __forceinline__ float carry(float A, float B, float s) {
+    constexpr int ZERO = 0x060, FINITE = 0x1f8;   // classes: -0, +0; these, denormal and normal ones
+    const bool none = __builtin_amdgcn_classf(s, fabsf(A) <= GONE ? FINITE : ZERO);
+    return none ? B : __builtin_fmaf(A, s, B);
+}
 
 // ---- a piece as one affine map of the state that enters it (BACK: from its far end)
 template <class T, int MODE, int V, bool UNI, bool NT, bool BACK>
@@ -322,9 +337,10 @@ __global__ __launch_bounds__(256) void k_scan_agg(ScanArgs p) {
     const Seg g = seg_of(p, s);
     if (g.first >= g.end) return;
     if (BACK ? g.first == g.base : g.end == g.stop) return;   // nothing follows it
-    float A[V], B[V];
+    Gates<MODE> A[V];
+    float B[V];
 #pragma unroll
-    for (int v = 0; v < V; v++) { A[v] = 1.0f; B[v] = 0.0f; }
+    for (int v = 0; v < V; v++) B[v] = 0.0f;
     const void *second = BACK ? p.dh : p.x;
     const int64_t ld2 = BACK ? p.ld_dh : p.ld_x;
     const int64_t nblk = (g.end - g.first + SB - 1) / SB;
@@ -355,7 +371,7 @@ __global__ __launch_bounds__(256) void k_scan_agg(ScanArgs p) {
 #pragma unroll
                 for (int v = 0; v < V; v++) {
                     B[v] = BACK ? a[v] * (b[v] + B[v]) : __builtin_fmaf(a[v], B[v], b[v]);
-                    A[v] = chain<MODE>(A[v], a[v]);
+                    A[v].take(a[v]);
                 }
             }
         }
@@ -364,14 +380,14 @@ __global__ __launch_bounds__(256) void k_scan_agg(ScanArgs p) {
     }
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        p.A[s * p.D + ch + v] = A[v];
+        p.A[s * p.D + ch + v] = A[v].all();
         p.B[s * p.D + ch + v] = B[v];
     }
 }
 
 // ---- the state that enters each piece, left in B.  One workgroup: 64 channels of one utterance, its pieces in CW runs of
 // consecutive ones; each wave reduces its run, the runs' maps are chained through LDS, and each wave walks its run again.  Bound by
-// the latency of that walk: 375 pieces of 1,024 channels (3 MB) 17 us.
+// the latency of that walk: 375 pieces of 1,024 channels (3 MB) 18 us.
 static constexpr int CW = 16;
 
 template <bool BACK>
@@ -385,14 +401,15 @@ __global__ __launch_bounds__(64 * CW) void k_scan_carry(ScanArgs p) {
     const bool on = ch < p.D;
     const int64_t per = (m + CW - 1) / CW, k0 = w * per, k1 = k0 + per < m ? k0 + per : m;
     auto at = [&](int64_t k) { return (s0 + (BACK ? m - 1 - k : k)) * p.D + ch; };
-    float A = 1.0f, B = 0.0f;
+    Gates<SRX_SCAN_VALUE> A;
+    float B = 0.0f;
     if (on)
         for (int64_t k = k0; k < k1 && k < m - 1; k++) {   // the last piece's map is never needed (and not there)
             const float a = p.A[at(k)], b = p.B[at(k)];
             B = carry(a, b, B);
-            A = chain<SRX_SCAN_VALUE>(A, a);
+            A.take(a);
         }
-    la[w][lane] = A;
+    la[w][lane] = A.all();
     lb[w][lane] = B;
     __syncthreads();
     if (!on) return;

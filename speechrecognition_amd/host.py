@@ -21,6 +21,15 @@ def _ptr(a):
     return a.ctypes.data_as(C.c_void_p)
 
 
+def _scores_ptr(ctx, a):
+    """Address of emission scores: a DevArray, or an f32 torch tensor on the context's device."""
+    if hasattr(a, "ptr"):
+        return a.ptr
+    if _typed(a) != _capi.SRX_F32 or a.get_device() != ctx.device:
+        _refuse("emission scores", a, f"f32 on device {ctx.device}")
+    return a.data_ptr()
+
+
 class Context:
     """srx_ctx: one per GPU.  `stream` is a raw hipStream_t handle (int), 0 being the device's default stream, or None: a stream of
     the context's own.  torch.cuda.current_stream().cuda_stream puts the calls in order with torch's work on that stream; against a
@@ -419,7 +428,7 @@ class HmmBatch:
 
     def viterbi(self, emis_d, stride_t, stride_g=1, beam=1e10, path_d=None, final_d=None, status_d=None, noalloc=False):
         """hmm::viterbi for every utterance (src/hmm.cpp:150-224); emission (t, col) at
-        emis[t*stride_t + col*stride_g] (frame-major [T, G]: (G, 1); state-major [G, T]: (1, T)).
+        emis[t*stride_t + col*stride_g] (frame-major [T, G]: (G, 1); state-major [G, T]: (1, T)); a DevArray or a torch tensor.
         noalloc: srx_viterbi_batch_noalloc_dev (back-pointers in the library's fixed per-GPU array; the caller should
         then pass the three output buffers too, or this wrapper allocates them)."""
         ctx = self.ctx
@@ -427,7 +436,7 @@ class HmmBatch:
         final_d = final_d or ctx.zeros((max(self.n_utt, 1),), np.float32)
         status_d = status_d or ctx.zeros((max(self.n_utt, 1),), np.int32)
         fn = ctx.lib.srx_viterbi_batch_noalloc_dev if noalloc else ctx.lib.srx_viterbi_batch_dev
-        check(fn(ctx.h, C.byref(self.c), emis_d.ptr, stride_t, stride_g, beam, path_d.ptr, final_d.ptr, status_d.ptr), ctx.h)
+        check(fn(ctx.h, C.byref(self.c), _scores_ptr(ctx, emis_d), stride_t, stride_g, beam, path_d.ptr, final_d.ptr, status_d.ptr), ctx.h)
         return path_d, final_d, status_d
 
     def train_transition_probabilities(self, path_d, status_d):
@@ -536,7 +545,7 @@ class GraphHmm:
         n = len(frame_off) - 1
         path_d = ctx.zeros((max(int(frame_off[-1]), 1),), np.int32)
         final_d, fs_d, st_d = ctx.zeros((max(n, 1),), np.float32), ctx.zeros((max(n, 1),), np.int32), ctx.zeros((max(n, 1),), np.int32)
-        check(ctx.lib.srx_viterbi_graph_dev(ctx.h, self.h, emis_d.ptr, stride_t, stride_g, _ptr(frame_off), n, beam, final_mode,
+        check(ctx.lib.srx_viterbi_graph_dev(ctx.h, self.h, _scores_ptr(ctx, emis_d), stride_t, stride_g, _ptr(frame_off), n, beam, final_mode,
                                             path_d.ptr, final_d.ptr, fs_d.ptr, st_d.ptr), ctx.h)
         ctx.sync()
         return path_d.get(), final_d.get(), fs_d.get(), st_d.get()

@@ -1,0 +1,23 @@
+"""Every command of the repository that compiles device code leaves packed f32 instructions out."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+FLAG = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+
+
+def test_every_compile_command_has_the_flag():
+    found = 0
+    for folder, _, files in os.walk(ROOT):
+        if os.path.relpath(folder, ROOT).split(os.sep)[0] not in (".", "speechrecognition_amd", "tools", "tests", "oracle"):
+            continue
+        for name in files:
+            if not (name == "Makefile" or name.endswith((".sh", ".hip"))):
+                continue
+            text = open(os.path.join(folder, name)).read().replace("\\\n", " ")
+            for line in re.findall(r".*(?:hipcc -|HIPCC\)|HIPFLAGS *:=).*", text):
+                if "HIPFLAGS)" in line or "-shared" in line:
+                    continue
+                found += 1
+                assert FLAG in line, (name, line)
+    assert found >= 3

@@ -10,8 +10,8 @@ C=speechrecognition_amd/csrc
 H=speechrecognition_amd/host
 for f in $C/srx_*.hip; do
     o=$OUT/obj/$(basename ${f%.hip}).o
-    if [ ! -f $o ] || [ $f -nt $o ]; then
-        /opt/rocm/bin/hipcc -O1 -g -std=c++17 --offload-arch=gfx950 -fPIC -ffp-contract=off -fno-fast-math -Wno-unused-result \
+    if [ ! -f $o ] || [ $f -nt $o ] || [ tools/build_host_asan.sh -nt $o ]; then
+        /opt/rocm/bin/hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O1 -g -std=c++17 --offload-arch=gfx950 -fPIC -ffp-contract=off -fno-fast-math -Wno-unused-result \
             -Xarch_host -fsanitize=address -Xarch_host -fsanitize=undefined -Xarch_host -fno-omit-frame-pointer -c $f -o $o &
     fi
 done

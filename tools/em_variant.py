@@ -2,7 +2,7 @@
 """Kernel A/B helper: times k_em_fused (one-pass EM statistics) of one or more builds of libsrx on a synthetic alignment of
 20 M frames (state runs of ~12 frames, 2,000 states x 16 components x 39 dims), without looking at the results (diagnostic
 builds may compute garbage).  Development tool only.
-  hipcc ... -DSRX_FUSED_EXP_<X> -c srx_train_seg.hip -o /tmp/v.o && link against the other objects -> python tools/em_variant.py lib1.so lib2.so"""
+  hipcc <HIPFLAGS of csrc/Makefile> -DSRX_FUSED_EXP_<X> -c srx_train_seg.hip -o /tmp/v.o && link against the other objects -> python tools/em_variant.py lib1.so lib2.so"""
 import os
 import sys
 

@@ -1,7 +1,7 @@
 // Microbenchmark: issue cost (SIMD cycles per wave instruction) of the f64 / conversion instructions the statistics kernels
 // are made of, on gfx950: eight independent chains per lane, one wave per SIMD slot (WAVES waves per workgroup of one CU-full
 // grid), s_memtime around a long unrolled loop.  Development tool (not part of libsrx).
-//   hipcc -O3 --offload-arch=gfx950 tools/microbench/f64_rates.hip -o gpurun_tmp/f64_rates && gpurun_tmp/f64_rates
+//   hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O3 --offload-arch=gfx950 tools/microbench/f64_rates.hip -o gpurun_tmp/f64_rates && gpurun_tmp/f64_rates
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

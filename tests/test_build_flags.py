@@ -21,3 +21,17 @@ def test_every_compile_command_has_the_flag():
                 found += 1
                 assert FLAG in line, (name, line)
     assert found >= 3
+
+
+def test_build_compiles_what_is_built_already(monkeypatch):
+    import subprocess
+    import sys
+
+    sys.path.insert(0, ROOT)
+    import __graft_entry__ as entry
+    from speechrecognition_amd import _capi
+    commands = []
+    monkeypatch.setattr(subprocess, "check_call", commands.append)
+    monkeypatch.setattr(_capi, "load", lambda: None)
+    entry.build()
+    assert len(commands) == 3 and all("-B" in c for c in commands)

@@ -41,7 +41,8 @@ typedef struct srx_ctx srx_ctx;
 /* ---------------------------------------------------------------- context ---------- */
 /* One per GPU.  `stream` is a hipStream_t to launch on (NULL: the context creates its own, which waits for no other stream and
  * which no other stream waits for).  SRX_STREAM_DEFAULT: the device's default stream, whose handle is NULL -- the one that torch works
- * on unless told otherwise; calls are then ordered with that work, and nothing else is needed. */
+ * on unless told otherwise; calls are then ordered with that work, and nothing else is needed.  Its calls cannot be captured into
+ * a graph. */
 #define SRX_STREAM_DEFAULT ((void *)1)
 int srx_ctx_create(int device, void *stream, srx_ctx **out);
 void srx_ctx_destroy(srx_ctx *ctx);
@@ -478,9 +479,9 @@ typedef enum { SRX_F32 = 0, SRX_F16 = 1, SRX_BF16 = 2 } srx_dtype;
  * gate, x, h: [total_frames][ld >= D] of `dtype`; h0, h_last: [n_utt][D] f32.  The state is f32 throughout.
  * max_frames: the longest utterance where the caller knows it (0: unknown); it only chooses how the work is cut.
  * states_dev: srx_gated_scan_states_len floats that the backward pass reads (the state in front of every
- * SRX_SCAN_STATE_EVERY-th frame), or NULL.  scratch_dev: srx_gated_scan_scratch_bytes (which may be 0), for either pass; it
- * holds nothing between calls.  At most 2^40 frames, 2^20 channels, and 2^25 utterances times 64 channels (2^22 utterances where
- * they are cut).  Where an utterance is cut into pieces its state passes a piece through the product of the
+ * SRX_SCAN_STATE_EVERY-th frame), or NULL.  scratch_dev: srx_gated_scan_scratch_bytes (which may be 0, and does not grow
+ * evenly with the sizes: ask for each), for either pass; it holds nothing between calls.  At most 2^40 frames, 2^20 channels,
+ * and 2^25 utterances times 64 channels (2^22 utterances where they are cut).  Where an utterance is cut into pieces its state passes a piece through the product of the
  * piece's gates: for gates beyond +-1 that product has to stay inside the f32 range.  Infinities pass a piece as they pass its
  * frames one by one. */
 enum { SRX_SCAN_VALUE = 0, SRX_SCAN_SIGMOID = 1 };
@@ -500,9 +501,9 @@ int srx_gated_scan_backward_dev(srx_ctx *ctx, int mode, int dtype, const void *g
                                 void *dgate_dev, int64_t ld_dgate, void *dx_dev, int64_t ld_dx, float *dh0_dev, void *scratch_dev,
                                 int64_t scratch_bytes);
 
-/* Matrix products whose weights change from group to group of rows (speakers, utterances, phone classes; beside
- * alignment-mode scoring, where every utterance meets its own states).  Group e owns rows [row_off[e], row_off[e+1]) (DEVICE
- * array of n_groups + 1 entries, frame_off's form); a group may have none.  W: [n_groups][N][K] contiguous, of the rows' type.
+/* Matrix products whose weights change from group to group of rows (speakers, utterances, or classes that the caller has sorted the
+ * rows by; beside alignment-mode scoring, where every utterance meets its own states).  Group e owns rows
+ * [row_off[e], row_off[e+1]) (DEVICE array of n_groups + 1 entries, frame_off's form); a group may have none.  W: [n_groups][N][K] contiguous, of the rows' type.
  *   srx_group_matmul_dev      y_r = W_e x_r + b_e            x [total_rows][ld >= K] -> y [total_rows][ld >= N]; bias [n_groups][N] f32 or NULL
  *   srx_group_matmul_dx_dev   dx_r = W_e^T dy_r              dy [total_rows][ld >= N] -> dx [total_rows][ld >= K]
  *   srx_group_matmul_dw_dev   dW_e = sum dy_r x_r^T          -> dw [n_groups][N][K], zeros for a group of no rows;
@@ -522,9 +523,9 @@ int srx_group_matmul_dw_dev(srx_ctx *ctx, int in_dtype, int out_dtype, const voi
 
 /* 8-bit matrix product with a scale for each row and each output (beside srx_gmm_score_dev: emission scores of an output layer
  * over the tied states, in the strides that srx_viterbi_* reads).
- * srx_quantize_rows_dev (less than 2^26 rows; of more than 4 KiB each: at most 2^26 - 4): scale_r = max_k |x_rk| / 127 (f32), q_rk = x_rk / scale_r (f32 quotient) rounded
- *   to the nearest whole number, ties to even; a row of zeros has scale 0 and codes 0 (and where the scale lies below the normal
- *   range, codes are held to +-127); a row that holds a NaN or an infinity has that as its scale and codes 0, so that its outputs
+ * srx_quantize_rows_dev (less than 2^26 rows; of more than 4 KiB each: at most 2^26 - 4): scale_r = max_k |x_rk| / 127 (f32),
+ *   q_rk = x_rk / scale_r (f32 quotient) rounded to the nearest whole number, ties to even; a row of zeros has scale 0 and codes 0 (and
+ *   where the scale lies below the normal range, codes are held to +-127); a row that holds a NaN or an infinity has that as its scale and codes 0, so that its outputs
  *   are NaN.  x: [rows][ld >= K] of `dtype`; codes: [rows][ld_q], ld_q a multiple of 16 bytes,
  *   q_dev 16-byte aligned, zeros written behind column K up to whole 16 bytes.  Weights (rows = outputs) are quantised by the
  *   same call, once.

@@ -376,7 +376,9 @@ static int group_check(srx_ctx *ctx, const char *name, int in_dtype, int out_dty
 
 // 32 x 32 tiles: for groups of few rows on average (the product is bound by reading W once), and where even these tiles are no
 // more than the chip holds at a time (two to a CU): the larger ones would leave most of it idle, each with a long reduction
-// before it (345 rows x 1,370 -> 1 f32: 66 us as 3 tiles of 128 rows, 15 us as 11 of 32 with 8 waves to a reduction).
+// before it (345 rows x 1,370 -> 1 f32: 66 us as 3 tiles of 128 rows, 15 us as 11 of 32 with 8 waves to a reduction).  The groups'
+// sizes are on the device, so the rule sees their mean: many groups of one row beside a long one lose (500 x 1 and 15,000 rows, 512 ->
+// 512 bf16: 163 us, 63 in the larger tiles).
 static constexpr int64_t THIN_ROWS = 32;
 static bool group_thin(const srx_ctx *ctx, int64_t total, int E, int N) {
     return total <= THIN_ROWS * E || (total / 32 + E) * ceil_div64(N, 32) <= 2 * (int64_t)ctx->num_cus;

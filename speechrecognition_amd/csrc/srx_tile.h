@@ -20,8 +20,9 @@
 // Bound by the matrix cores and what stands beside them: a workgroup of 256 x 256 fills a CU's LDS and half its registers, so its first
 // loads and its stores run beside nobody's products (8 groups, 65,536 rows, 1,024 x 1,024 bf16: matrix cores busy 0.49 of the time,
 // forward 170 us or 810 TFLOP/s; 16,384 x 4,096 x 4,096: 1,087).  Tried and slower: slabs of 64 bytes four or five deep (10 %),
-// touching the slab after next for the L2 (15 %), four waves of 128 x 128, workgroups that stay and take tile after tile (loads
-// wait behind the stores of the tile before them: the counter of memory operations is in order).
+// touching the slab after next for the L2 (15 %), four waves of 128 x 128.  Workgroups that stay and take tile after tile were slower
+// on the f32 39 -> 39 transform (113 us, 86 then; loads wait behind the stores of the tile before them: the counter of memory
+// operations is in order) and are not measured on these tiles.
 //
 // Result layout: lane l holds column j = l & 31, rows 8 b + 4 (l >> 5) + 0..3 for b = 0..3: four adjacent i for one j.
 #pragma once
@@ -571,7 +572,8 @@ __device__ __forceinline__ void tile_of(int64_t b, int64_t ni, int64_t nj, int64
 
 // Tile of 256 x 256 on 8 waves or of 128 x 128 on 4?  A CU holds one of the former or two of the latter.  A round of the small
 // ones costs 0.63 of a round of the large (8 groups, 65,536 rows, 1,024 x 1,024 bf16: 20.8 us and 33 us; 165 us against 187 us in
-// all); few tiles are better spread over the chip as small ones.
+// all); few tiles are better spread over the chip as small ones.  Fitted at that reduction of 16 slabs only: where the slabs are few
+// (429 8-bit elements: 4) a tile's stores weigh more than the rule knows.
 static inline bool tile_large(int64_t large, int64_t small, int64_t cus) {
     return ceil_div64(large, cus) * 100 <= ceil_div64(small, 2 * cus) * 63;
 }

@@ -14,7 +14,7 @@ def test_every_compile_command_has_the_flag():
         for name in files:
             if not (name == "Makefile" or name.endswith((".sh", ".hip"))):
                 continue
-            text = open(os.path.join(folder, name)).read().replace("\\\n", " ")
+            text = open(os.path.join(folder, name), encoding="utf-8").read().replace("\\\n", " ")
             for line in re.findall(r".*(?:hipcc -|HIPCC\)|HIPFLAGS *:=).*", text):
                 if "HIPFLAGS)" in line or "-shared" in line:
                     continue
